@@ -224,6 +224,39 @@ MOTIF_API int motif_vanilla_decode_step(const void* qkv, const float* inv_freq, 
                                         float eps, void* out, void* workspace, size_t workspace_bytes,
                                         void* stream);
 
+/* ---- attention for a tree of drafted tokens ---------------------------------
+ * motif_sdpa_dual_v for the T = tree_rows query rows of a verify forward over
+ * a tree (or several chains) of drafted tokens: q (B, h_q, T, D), y
+ * (B, h_q, T, 2D). The keys and values of tree row j are cache row
+ * n - T + j, n = the live rows kv_len (the tree's rows appended); query row t
+ * sees every cache row below n - T and the tree rows j with tree_mask[t, j]
+ * set ((T, T) bytes, or (B, T, T) with mask_batch_stride = T * T; NULL: causal,
+ * j <= t). A row that sees nothing gives 0; rows >= n are never used, and a
+ * tree row hidden from a query does not reach it even if it holds NaN. No
+ * counterpart in the reference (its verify forward is one chain, run as a
+ * causal prompt block).
+ * kv: k, v1, v2. bits 16: rows in dtype, stride = elements between batches,
+ * heads and rows (multiples of 16 bytes; the channels are contiguous). bits 4
+ * or 8: contiguous MLX affine triples, group_size a multiple of 8 that divides
+ * D (stride unused). D 64 or 128, T <= 256.
+ * kv_len_dev: one length (kv_len_stride 0) or one per sequence (1), clamped to
+ * [0, kv_cap]; with fewer than T live rows the tree's first rows are missing.
+ * workspace: motif_sdpa_dual_v_tree_workspace_bytes(D), any contents; calls
+ * that may overlap need one each. err (optional device int): set to 1 if a
+ * pipeline wait timed out (the rows it concerns are then NaN). */
+typedef struct motif_tree_kv {
+  const void* data[3];
+  const void* scales[3];
+  const void* biases[3];
+  int64_t stride[3];
+} motif_tree_kv;
+MOTIF_API size_t motif_sdpa_dual_v_tree_workspace_bytes(int64_t head_dim);
+MOTIF_API int motif_sdpa_dual_v_tree(int dtype, int bits, int group_size, const void* q, const motif_tree_kv* kv,
+                                     const uint8_t* tree_mask, int64_t mask_batch_stride, float scale, int64_t batch,
+                                     int64_t h_q, int64_t h_kv, int64_t tree_rows, int64_t kv_cap, int64_t head_dim,
+                                     int64_t kv_len, const int32_t* kv_len_dev, int64_t kv_len_stride, void* y,
+                                     void* workspace, size_t workspace_bytes, int* err, void* stream);
+
 /* Which kernel motif_gda_decode_step / motif_vanilla_decode_step launch for
  * this cache (no reference counterpart: the reference has one Metal kernel
  * per dtype, kernels/attention.py:190-260 and 510-645). Returns
@@ -259,6 +292,22 @@ MOTIF_API int motif_dequantize(int dtype, int bits, int group_size, const uint32
 MOTIF_API int motif_kv4_append(int dtype, const motif_kv4_slots* cache, const void* k1, const void* k2,
                      const void* v1, const void* v2, int64_t seq, int64_t offset,
                      const int32_t* offset_dev, void* stream);
+
+/* After a tree of tree_rows rows was appended at rows [base, base + tree_rows)
+ * and verified: row base + path[j] moves to row base + j for j = 1 ..
+ * accepted, in the four slots of n_caches caches of one geometry (the layers),
+ * one launch for up to 64 of them. path (B, tree_rows) and accepted (B) as
+ * motif_speculative_verify writes them (path ascends from path[0] = 0);
+ * entries that are not above j or not below tree_rows move nothing, and
+ * accepted is clamped to [0, tree_rows). base_dev: one base for all sequences
+ * (base_stride 0) or one each (1), read on the device; rows at or beyond row_limit
+ * (the rows a head really has: the capacity, or less where a view's heads
+ * interleave) are not touched. dtype: the rows' (bits 16) or the scales' type. The
+ * reference only trims a rejected tail (cache.py:297-300): its drafts are
+ * chains, whose accepted rows are in place already. */
+MOTIF_API int motif_kv4_keep_rows(int dtype, const motif_kv4_slots* caches, int64_t n_caches, const int32_t* path,
+                                  int64_t path_batch_stride, const int32_t* accepted, int64_t tree_rows, int64_t base,
+                                  const int32_t* base_dev, int64_t base_stride, int64_t row_limit, void* stream);
 
 /* Decode prologue of _forward_grouped (model.py:580-657) for batch 1, S = 1:
  * split the fused qkv row (q_heads + 2*kv2 + 2*kv2 heads of D, Q origin-first,
@@ -528,6 +577,34 @@ MOTIF_API int motif_sample_key(const void* logits, int64_t n, float temperature,
 MOTIF_API int motif_speculative_accept(const void* p_logits, const void* q_logits, int64_t row_stride,
                                        const int32_t* draft_tokens, int64_t k, int64_t n, float temperature,
                                        uint64_t seed, const int32_t* pos_dev, int64_t pos_host, int32_t* out,
+                                       void* stream);
+
+/* Verification of a tree (or chain) of drafted tokens from given uniforms, for
+ * a batch of sequences. Row 0 is the last committed token, row i >= 1 the
+ * drafted token tokens[b, i] with parent row parents[i] < i ((rows) for all
+ * sequences, or (B, rows) with parents_batch_stride = rows). p_logits: the
+ * target's row after tree row r; q_logits: the draft's row r, from which row
+ * r's children were drawn independently (draft_rows rows: only rows with
+ * children are read; a row without a draft row accepts no child). Starting at
+ * row 0 the children of the current row are tested in ascending order with
+ * uniforms[b, i]: accepted with probability min(1, w(x) / q(x)), w = p and
+ * after each rejection max(0, w - q) renormalised; an accepted child becomes
+ * the current row. next_token is drawn from the last w by inverting its
+ * running sum at uniforms[b, 0]: the tokens follow the target's law. Temperature
+ * 0: a child is accepted if it is the target's argmax, next_token = the argmax
+ * (first index on ties); q_logits and uniforms may be NULL. A token outside
+ * [0, vocab) is never accepted (padding); NaN logits count as -inf; a target
+ * row without a finite logit accepts nothing and yields token 0.
+ * accepted (B): drafted tokens accepted; path (B, rows): 0, the accepted rows,
+ * then -1. Strides in elements. The reference's rule for one chain with its
+ * own random numbers is motif_speculative_accept's. */
+MOTIF_API size_t motif_speculative_verify_workspace_bytes(int64_t batch, int64_t rows, int64_t draft_rows);
+MOTIF_API int motif_speculative_verify(int dtype, const void* p_logits, int64_t p_batch_stride, int64_t p_row_stride,
+                                       const void* q_logits, int64_t q_batch_stride, int64_t q_row_stride,
+                                       int64_t draft_rows, const int32_t* tokens, const int32_t* parents,
+                                       int64_t parents_batch_stride, const float* uniforms, int64_t batch,
+                                       int64_t rows, int64_t vocab, double temperature, int32_t* accepted,
+                                       int32_t* path, int32_t* next_token, void* workspace, size_t workspace_bytes,
                                        void* stream);
 
 /* Greedy sampler: first index of the maximum of logits (n,) -> *out_index

@@ -12,6 +12,7 @@ other misuse ``ValueError``/``TypeError``, CUDA failures ``RuntimeError``.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 from pathlib import Path
@@ -78,9 +79,19 @@ class motif_linear_io(C.Structure):  # noqa: N801 — mirrors the C struct name
     ]
 
 
+class motif_tree_kv(C.Structure):  # noqa: N801 — mirrors the C struct name
+    _fields_ = [
+        ("data", C.c_void_p * 3),
+        ("scales", C.c_void_p * 3),
+        ("biases", C.c_void_p * 3),
+        ("stride", C.c_int64 * 3),
+    ]
+
+
 _P, _I, _L, _F, _S = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_size_t
 _KV = C.POINTER(motif_kv4_slots)
 _IO = C.POINTER(motif_linear_io)
+_TKV = C.POINTER(motif_tree_kv)
 
 # name -> (restype, argtypes); every symbol of include/motif_b200.h.
 SIGNATURES = {
@@ -142,6 +153,17 @@ SIGNATURES = {
     "motif_argmax": (_I, [_I, _P, _L, _P, _P, _S, _P]),
     "motif_argmax_key_decode": (_I, [_P, _P, _P, _P]),
     "motif_argmax_key_exchange": (_I, [_P, _P, _I, _I, _P, _P, _P, _P, _P]),
+    "motif_sdpa_dual_v_tree_workspace_bytes": (_S, [_L]),
+    "motif_sdpa_dual_v_tree": (
+        _I,
+        [_I, _I, _I, _P, _TKV, _P, _L, _F, _L, _L, _L, _L, _L, _L, _L, _P, _L, _P, _P, _S, _P, _P],
+    ),
+    "motif_kv4_keep_rows": (_I, [_I, _KV, _L, _P, _L, _P, _L, _L, _P, _L, _L, _P]),
+    "motif_speculative_verify_workspace_bytes": (_S, [_L, _L, _L]),
+    "motif_speculative_verify": (
+        _I,
+        [_I, _P, _L, _L, _P, _L, _L, _L, _P, _P, _L, _P, _L, _L, _L, C.c_double, _P, _P, _P, _P, _S, _P],
+    ),
     "motif_ipc_handle_bytes": (_S, []),
     "motif_ipc_alloc": (_I, [_S, C.POINTER(C.c_void_p), _P]),
     "motif_ipc_open": (_I, [_P, C.POINTER(C.c_void_p)]),
@@ -205,6 +227,15 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def stream(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def on_device(device: torch.device):
+    """A context in which ``device`` (a CUDA device) is the current one: launches go to its streams."""
+    if device.type != "cuda":
+        raise ValueError("mlx_motif kernels take CUDA tensors (got a CPU tensor)")
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def contiguous(t: torch.Tensor) -> torch.Tensor:

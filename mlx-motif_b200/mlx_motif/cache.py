@@ -24,7 +24,7 @@ from __future__ import annotations
 
 import torch
 
-from ._native import check, dtype_code, lib, motif_kv4_slots, ptr, stream
+from ._native import check, dtype_code, lib, motif_kv4_slots, on_device, ptr, stream
 
 
 def create_causal_mask(N: int, offset: int = 0, window_size: int | None = None) -> torch.Tensor:
@@ -64,6 +64,77 @@ def _slots_struct(slots, bits: int, group_size: int, B: int, H: int, cap: int, D
     s.capacity = cap
     s.head_dim = D
     return s
+
+
+def _filled(slots) -> list:
+    if any(s is None for s in slots):
+        raise ValueError("the cache is empty: append rows before taking its slots")
+    return list(slots)
+
+
+class KVSlots:
+    """C-ABI views of the caches of one model (its layers), for calls that serve them all at once. Holds
+    the buffers it was built over; build it again after a cache has grown or taken a new state."""
+
+    def __init__(self, caches):
+        caches = list(caches)
+        if not caches:
+            raise ValueError("kv_slots: no caches")
+        self.buffers = [c._buffers() for c in caches]
+        first = self.buffers[0][-1]  # a row or scale buffer: its type and device are the cache's
+        for bufs in self.buffers:
+            for t in bufs:
+                if t.device != first.device:
+                    raise ValueError(f"caches on {t.device} and {first.device}: all must be on one CUDA device")
+            if bufs[-1].dtype != first.dtype:
+                raise TypeError(f"caches of {bufs[-1].dtype} and {first.dtype}: all must have one type")
+        self.device = first.device
+        self.dtype_code = dtype_code(first)
+        self.structs = (motif_kv4_slots * len(caches))(*(c.slots_struct() for c in caches))
+        s = self.structs[0]
+        self.batch, self.capacity = s.batch, min(c._row_capacity() for c in caches)
+
+    def __len__(self) -> int:
+        return len(self.structs)
+
+
+def kv_slots(caches) -> KVSlots:
+    """The views of ``caches`` (filled caches of one geometry) that :func:`keep_rows` takes."""
+    return KVSlots(caches)
+
+
+def keep_rows(slots: KVSlots, path: torch.Tensor, accepted: torch.Tensor, base) -> None:
+    """Move the accepted rows of a verified tree to the front of the tree's rows, in every cache of ``slots``.
+
+    The tree's T rows were appended at cache rows [base, base + T); for j = 1 .. accepted[b], row
+    base + path[b, j] moves to row base + j in all four slots (k1, k2, v1, v2; codes, scales and biases of a
+    packed cache). path (B, T) and accepted (B,) int32 as ``speculative_verify`` returns them: path ascends
+    from path[:, 0] = 0 (entries not above j or not below T move nothing). ``base``: an int, or an int32 CUDA
+    tensor of one base or one per sequence. One launch (per 64 caches), nothing is read back; afterwards the
+    live rows are base + 1 + accepted[b]: with the count on the host, ``trim(T − 1 − accepted)``.
+    """
+    dev, B = slots.device, slots.batch
+    for t, name in ((path, "path"), (accepted, "accepted")):
+        if t.dtype != torch.int32:
+            raise TypeError(f"{name} must be int32, got {t.dtype}")
+        if t.device != dev:
+            raise ValueError(f"{name} on {t.device}, the caches on {dev}")
+    assert path.dim() == 2 and path.shape[0] == B, f"path {tuple(path.shape)} must be ({B}, T)"
+    assert tuple(accepted.shape) == (B,), f"accepted {tuple(accepted.shape)} must be ({B},)"
+    T = path.shape[1]
+    base_dev, base_step, base_host = None, 0, 0
+    if isinstance(base, torch.Tensor):
+        if base.dtype != torch.int32 or base.device != dev or base.numel() not in (1, B) or not base.is_contiguous():
+            raise TypeError(f"a device base must be a contiguous int32 tensor of 1 or {B} elements on {dev}")
+        base_dev, base_step = ptr(base), int(base.numel() > 1)
+    else:
+        base_host = int(base)
+        assert 0 <= base_host and base_host + T <= slots.capacity, \
+            f"rows [{base_host}, {base_host + T}) outside capacity {slots.capacity}"
+    with on_device(dev):
+        path, accepted = path.contiguous(), accepted.contiguous()
+        check(lib.motif_kv4_keep_rows(slots.dtype_code, slots.structs, len(slots.structs), ptr(path), T, ptr(accepted),
+                                      T, base_host, base_dev, base_step, slots.capacity, stream(dev)), "keep_rows")
 
 
 class MotifGroupedKVCacheBase:
@@ -130,6 +201,14 @@ class MotifGroupedKVCacheBase:
         """C-ABI view of the four slots (valid until the next growth)."""
         return self._struct()
 
+    def keep_rows(self, path: torch.Tensor, accepted: torch.Tensor, base=None) -> None:
+        """:func:`keep_rows` on this cache alone; ``base`` defaults to the first of the last T rows
+        (``offset − T``), the tree appended last."""
+        keep_rows(KVSlots([self]), path, accepted, self.offset - path.shape[1] if base is None else base)
+
+    def _row_capacity(self) -> int:
+        return self._slot_capacity(self.k1)
+
 
 class MotifGroupedKVCache(MotifGroupedKVCacheBase):
     """fp16/bf16 4-slot cache; each slot (B, H, capacity, D)."""
@@ -141,6 +220,9 @@ class MotifGroupedKVCache(MotifGroupedKVCacheBase):
 
     def _slot_capacity(self, slot) -> int:
         return slot.shape[2]
+
+    def _buffers(self) -> list:
+        return _filled((self.k1, self.k2, self.v1, self.v2))
 
     def _init_storage(self, B, H, n, D, dtype, device):
         return torch.zeros((B, H, n, D), dtype=dtype, device=device)
@@ -213,6 +295,9 @@ class MotifGroupedQuantizedKVCache(MotifGroupedKVCacheBase):
 
     def _slot_capacity(self, slot) -> int:
         return slot[0].shape[2]
+
+    def _buffers(self) -> list:
+        return [t for slot in _filled((self.k1, self.k2, self.v1, self.v2)) for t in slot]
 
     def _init_storage(self, B, H, n, D, dtype, device):
         el = 32 // self.bits
@@ -472,6 +557,14 @@ class KVCache:
         s.data[1] = s.data[1] + row_bytes
         s.data[3] = s.data[3] + row_bytes
         return s
+
+    keep_rows = MotifGroupedKVCacheBase.keep_rows
+
+    def _buffers(self) -> list:
+        return _filled((self.keys, self.values))
+
+    def _row_capacity(self) -> int:
+        return self.keys.shape[2]
 
     def update_and_fetch(self, keys, values):
         """Append (B, n_kv_heads, S, D) keys/values at ``offset``; return the live rows."""

@@ -8,6 +8,8 @@ a correctness mode.
     attention.py — sdpa_dual_v, sdpa_dual_v_q4  (shared-QK dual-V SDPA)
     gda.py       — gda_post, gda_post_split     (GDA post-attention reduction)
     mlp.py       — polynorm, polynorm_mul, _dequant_probe
+    tree.py      — sdpa_dual_v_tree, sdpa_dual_v_tree_q4  (a tree of drafted tokens over a cache)
+    verify.py    — speculative_verify  (drafted tokens against the target's probabilities)
 """
 
 from .attention import (
@@ -29,6 +31,15 @@ from .mlp import (
     polynorm_reference,
 )
 
+from .tree import (
+    sdpa_dual_v_tree,
+    sdpa_dual_v_tree_q4,
+    sdpa_dual_v_tree_q4_reference,
+    sdpa_dual_v_tree_reference,
+    tree_mask_from_parents,
+)
+from .verify import VerifyResult, speculative_verify, speculative_verify_reference
+
 __all__ = [
     "polynorm",
     "polynorm_reference",
@@ -41,4 +52,12 @@ __all__ = [
     "sdpa_dual_v_reference",
     "sdpa_dual_v_q4",
     "sdpa_dual_v_q4_reference",
+    "sdpa_dual_v_tree",
+    "sdpa_dual_v_tree_reference",
+    "sdpa_dual_v_tree_q4",
+    "sdpa_dual_v_tree_q4_reference",
+    "tree_mask_from_parents",
+    "speculative_verify",
+    "speculative_verify_reference",
+    "VerifyResult",
 ]

@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import torch
 
-from .._native import _DISABLE, check, contiguous, dtype_code, lib, ptr, stream  # noqa: F401
+from .._native import _DISABLE, check, contiguous, dtype_code, lib, on_device, ptr, stream  # noqa: F401
 
 
 def as_f32_device(value, device) -> torch.Tensor:
