@@ -1598,6 +1598,19 @@ bool encode_tma_rows(CUtensorMap* m, const void* base, uint64_t inner_bytes, uin
                      swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
+bool encode_tma_heads(CUtensorMap* m, const void* base, uint64_t inner_bytes, const uint64_t (&rows_heads_batch)[3],
+                      const uint64_t (&stride_bytes)[3], uint32_t box_inner, uint32_t box_rows) {
+  EncodeTiledFn fn = encoder();
+  if (!fn) return false;
+  cuuint64_t dims[4] = {inner_bytes, rows_heads_batch[0], rows_heads_batch[1], rows_heads_batch[2]};
+  cuuint64_t strides[3] = {stride_bytes[0], stride_bytes[1], stride_bytes[2]};
+  cuuint32_t box[4] = {box_inner, box_rows, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace motif
 
 using namespace motif;

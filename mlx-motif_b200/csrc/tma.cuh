@@ -15,6 +15,11 @@ namespace motif {
 bool encode_tma_rows(CUtensorMap* m, const void* base, uint64_t inner_bytes, uint64_t rows, uint32_t box_inner,
                      uint32_t box_rows, bool swizzle128);
 
+// Host: a 4D byte view (batch × heads × rows × inner_bytes, any strides that are multiples of 16 bytes)
+// with a box of box_rows × box_inner bytes in the 128-byte swizzle; rows outside read as zeros (qlinear.cu).
+bool encode_tma_heads(CUtensorMap* m, const void* base, uint64_t inner_bytes, const uint64_t (&rows_heads_batch)[3],
+                      const uint64_t (&stride_bytes)[3], uint32_t box_inner, uint32_t box_rows);
+
 namespace tc {
 
 constexpr int kMbarPolls = 1 << 22;
@@ -60,6 +65,23 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
           dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
       : "memory");
+}
+
+// 4D tiled TMA load (no multicast) completing on an mbarrier.
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w,
+                                            uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];\n" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
+}
+
+// Contiguous copy of `bytes` (a multiple of 16, both addresses 16-byte aligned) completing on an mbarrier.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
 }
 
 // Generic-proxy shared-memory writes become visible to the async proxy (tensor core, TMA).
@@ -182,11 +204,12 @@ __device__ __forceinline__ uint64_t desc_mnmajor_sw128(uint32_t saddr, uint32_t 
   return d;
 }
 
-// Instruction descriptor of kind::f16 with fp16 A and B, fp32 accumulator; each operand K-major
+// Instruction descriptor of kind::f16 with fp16 (or both bf16) A and B, fp32 accumulator; each operand K-major
 // unless its *_mn_major flag is set.
-__host__ __device__ constexpr uint32_t idesc_f16_f32(int M, int N, bool b_mn_major = false, bool a_mn_major = false) {
+__host__ __device__ constexpr uint32_t idesc_f16_f32(int M, int N, bool b_mn_major = false, bool a_mn_major = false,
+                                                     bool bf16 = false) {
   return (1u << 4)                           // D format f32
-         | (0u << 7) | (0u << 10)            // A, B format f16
+         | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10)  // A, B format: f16 or bf16
          | ((a_mn_major ? 1u : 0u) << 15)    // A major-ness
          | ((b_mn_major ? 1u : 0u) << 16)    // B major-ness
          | ((uint32_t)(N >> 3) << 17)        // N / 8

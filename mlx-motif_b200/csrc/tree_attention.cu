@@ -13,9 +13,13 @@
 // (Schedule), whatever the sequences' lengths: a CTA may end one unit and start the next. A unit
 // that lies in one CTA is normalised and written by it; the others leave fp32 partials (running
 // maximum, Σp, unnormalised O) that tree_merge_kernel joins in a fixed order.
+#include <cuda.h>
+
 #include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
+#include "tma.cuh"
 
 namespace motif {
 namespace {
@@ -34,8 +38,9 @@ struct TreeArgs {
   int len_step;             // 0: one for all sequences
   int len;
   void* y;                  // (B, HKV·gqa, T, 2D)
-  float* part_o;            // [2·grid][tile rows][2D]
-  float* part_ml;           // [2·grid][tile rows][2]
+  float* part_o;            // [2·grid][slot_rows][2D]
+  float* part_ml;           // [2·grid][slot_rows][2]
+  int slot_rows;            // rows of a partial: min(tile_rows, R)
   int* err;
   int B, HKV, gqa, T, R, row_tiles, cap, gs;
   int tile_rows, tile_keys;
@@ -52,33 +57,25 @@ __device__ __forceinline__ int key_tiles(const TreeArgs& a, int n) {
 
 // Line of all units' key tiles, and this CTA's part [x, x1) of it. Every thread of a warp calls it.
 struct Schedule {
-  int64_t total, x, x1;
-  int b;         // sequence of x
-  int64_t base;  // its first tile
-  int n, nt;     // its live rows and key tiles per unit
+  int x0, x, x1;
+  int b, base;  // sequence of x, its first tile
+  int n, nt;    // its live rows and key tiles per unit
 
   __device__ __forceinline__ Schedule(const TreeArgs& a) {
     const int lane = threadIdx.x & 31;
     const int per_b = a.HKV * a.row_tiles;
-    int64_t s = 0;
-    for (int i = lane; i < a.B; i += 32) s += key_tiles(a, live_rows(a, i));
+    int total = 0;  // < 2^31: checked by the host for the longest lengths
+    for (int i = lane; i < a.B; i += 32) total += key_tiles(a, live_rows(a, i));
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    total = s * per_b;
-    x = lo(blockIdx.x, gridDim.x);
-    x1 = lo(blockIdx.x + 1, gridDim.x);
-    seek(a, x);
-  }
-  __device__ __forceinline__ int64_t lo(int64_t i, int64_t grid) const { return i * total / grid; }
-  // The sequence that holds tile `at` (at < total, or the last one).
-  __device__ __forceinline__ void seek(const TreeArgs& a, int64_t at) {
-    const int64_t per_b = (int64_t)a.HKV * a.row_tiles;
-    b = 0;
-    base = 0;
-    for (;;) {
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    total *= per_b;
+    x0 = x = (int)((int64_t)blockIdx.x * total / gridDim.x);
+    x1 = (int)((int64_t)(blockIdx.x + 1) * total / gridDim.x);
+    b = base = 0;
+    for (;;) {  // the sequence that holds tile x
       n = live_rows(a, b);
       nt = key_tiles(a, n);
-      if (b + 1 >= a.B || at < base + nt * per_b) return;
+      if (b + 1 >= a.B || x < base + nt * per_b) return;
       base += nt * per_b;
       ++b;
     }
@@ -88,30 +85,27 @@ struct Schedule {
 // One CTA's share of one unit: key tiles [t0, t1) of row tile rt of kv head g of sequence b.
 struct Segment {
   int b, g, rt, n, t0, t1;
-  bool whole;   // the unit lies in this CTA
-  int64_t slot; // its partial's place otherwise
+  int slot;    // its partial's place; -1: the unit lies in this CTA
 };
 
 __device__ __forceinline__ bool next_segment(const TreeArgs& a, Schedule& s, Segment& g) {
   if (s.x >= s.x1) return false;
-  const int64_t per_b = (int64_t)a.HKV * a.row_tiles;
+  const int per_b = a.HKV * a.row_tiles;
   if (s.x >= s.base + s.nt * per_b) {
     s.base += s.nt * per_b;
     ++s.b;
     s.n = live_rows(a, s.b);
     s.nt = key_tiles(a, s.n);
   }
-  const int64_t in = s.x - s.base;
-  const int u = (int)(in / s.nt);
+  const int in = s.x - s.base, u = in / s.nt;
   g.b = s.b;
   g.n = s.n;
   g.g = u / a.row_tiles;
   g.rt = u - g.g * a.row_tiles;
-  g.t0 = (int)(in - (int64_t)u * s.nt);
-  g.t1 = (int)min((int64_t)s.nt, g.t0 + (s.x1 - s.x));
-  g.whole = g.t0 == 0 && g.t1 == s.nt;
-  // at most two segments of a CTA are parts: the first (a unit begun before it) and the last
-  g.slot = 2 * (int64_t)blockIdx.x + (s.x == s.lo(blockIdx.x, gridDim.x) ? 0 : 1);
+  g.t0 = in - u * s.nt;
+  g.t1 = min(s.nt, g.t0 + (s.x1 - s.x));
+  // at most two segments of a CTA are parts of units: the first (a unit begun before it) and the last
+  g.slot = g.t0 == 0 && g.t1 == s.nt ? -1 : 2 * (int)blockIdx.x + (s.x == s.x0 ? 0 : 1);
   s.x += g.t1 - g.t0;
   return true;
 }
@@ -122,7 +116,7 @@ __device__ __forceinline__ uint64_t visible(const TreeArgs& a, int b, int t, int
   const int ctx = n - a.T;  // negative where fewer than T rows are live
   uint64_t w = 0;
   const uint8_t* m = a.mask ? a.mask + b * a.mask_b + (int64_t)t * a.T : nullptr;
-#pragma unroll
+#pragma unroll 16
   for (int c = 0; c < NB; ++c) {
     const int pos = p0 + c, j = pos - ctx;
     bool v = pos < n;
@@ -270,8 +264,8 @@ __global__ void __launch_bounds__(kSThreads, 2) tree_simt_kernel(const __grid_co
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         inv_l[2 * warp + h] = l[h] == 0.f ? 0.f : 1.f / l[h];
-        if (!sg.whole && 2 * warp + h < rows) {
-          float* ml = a.part_ml + (sg.slot * kSR + 2 * warp + h) * 2;
+        if (sg.slot >= 0 && 2 * warp + h < rows) {
+          float* ml = a.part_ml + ((int64_t)sg.slot * a.slot_rows + 2 * warp + h) * 2;
           ml[0] = m[h];
           ml[1] = l[h];
         }
@@ -281,12 +275,625 @@ __global__ void __launch_bounds__(kSThreads, 2) tree_simt_kernel(const __grid_co
 #pragma unroll
     for (int r = 0; r < kAcc; ++r) {
       if (row0 + r >= rows) break;
-      if (sg.whole)
+      if (sg.slot < 0)
         static_cast<T*>(a.y)[(qrow + row0 + r) * 2 * D + ch] = from_f<T>(acc[r] * inv_l[row0 + r]);
       else
-        a.part_o[(sg.slot * kSR + row0 + r) * 2 * D + ch] = acc[r];
+        a.part_o[((int64_t)sg.slot * a.slot_rows + row0 + r) * 2 * D + ch] = acc[r];
     }
   }
+}
+
+// ---- tensor-core form: 16-bit rows and packed caches of 16-bit models --------------------------------
+// One CTA per SM takes 128 packed query rows (rows past the unit's are zero) and 64-key tiles:
+//   S = Q·Kᵀ (M 128, N 64, K D) and O += P·[V1 | V2] (M 128, N 2D, K 64) run as tcgen05.mma into tensor
+// memory (S double-buffered: 2 × 64 columns, O: 2D columns); Q, K and P are K-major, V is MN-major as the
+// cache rows lie, all in the 128-byte swizzle.
+//   warp 0       TMA: K and V tiles straight from the cache into rings of kStages (16-bit rows), or the
+//                packed rows, scales and biases into a ring of raw tiles;
+//   warp 1       one lane issues the MMAs, S one tile ahead within a segment;
+//   warps 2..5   a thread is a query row: loads Q, takes S from tensor memory, keeps the running maximum
+//                and sum, writes P in the type; O is rescaled in tensor memory only when a row's maximum
+//                grew by more than 2^8 (weights stay ≤ 256, and the result is exact). Warps without a row
+//                only keep the barriers.
+//   warps 6..13  (packed) rebuild K and V tiles from the codes with packed 16-bit arithmetic: the code is
+//                exact in the type (exponent trick), scale·code + bias one fused rounding.
+// Where the tile holds drafted rows or the cache's end, the softmax warps clear V rows that no query may
+// use (rows ≥ n, whatever the buffer holds) and drafted rows with a non-finite value: a zero weight times
+// NaN would reach queries the row is hidden from. The queries that do see such a row add it at the end
+// from the cache itself.
+// Every wait is bounded; one that runs out sets the abort flag, rows not finished become NaN and the
+// error word is set, and the CTA drains its copies and MMAs before it frees tensor memory.
+constexpr int kTR = 128, kTK = 64;
+
+template <int BITS>
+struct TcCfg {
+  static constexpr int kStages = BITS == 16 ? 3 : 2;  // K/V operand tiles
+  static constexpr int kThreads = BITS == 16 ? 192 : 448;
+  static constexpr int kFill = BITS == 16 ? 1 : 8;  // arrivals that fill a K or V tile
+};
+constexpr int kRawMax = 4;
+
+struct TcArgs {
+  TreeArgs t;
+  CUtensorMap tm[3];  // k, v1, v2 rows
+  int raw_stages, code_bytes, group_bytes;  // packed: ring depth, bytes of a row's codes and of its scales
+};
+
+template <int D, int BITS>
+struct TcMap {  // shared memory, bytes from a 1024-byte boundary
+  static constexpr int kHalves = D / 64;
+  static constexpr int kQ = 0;
+  static constexpr int kK = kQ + kHalves * kTR * 128;
+  static constexpr int kKBytes = kHalves * kTK * 128;
+  static constexpr int kV = kK + TcCfg<BITS>::kStages * kKBytes;
+  static constexpr int kVBytes = 2 * kKBytes;
+  static constexpr int kP = kV + TcCfg<BITS>::kStages * kVBytes;
+  static constexpr int kBar = kP + 2 * kTR * 128;
+  static constexpr int kNumBars = 1 + 4 * TcCfg<BITS>::kStages + 4 + 2 + 2 * kRawMax;
+  static constexpr int kBad = kBar + kNumBars * 8 + 16;  // [2 segments][4 warps][8 words]: drafted rows cleared
+  static constexpr int kRaw = (kBad + 2 * 4 * 8 * 4 + 127) / 128 * 128;
+};
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Any of the two 16-bit values of w is an infinity or NaN.
+template <typename T>
+__device__ __forceinline__ bool nonfinite2(uint32_t w) {
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+  return (w & e) == e || ((w >> 16) & e) == e;
+}
+
+// Channel held at position i of an 8-channel chunk of the operand tiles: q4 words give the channel pairs
+// (j, j + 4) in one instruction, so K, V and Q keep that order and the output undoes it.
+template <int BITS>
+__host__ __device__ constexpr int chunk_channel(int i) {
+  return BITS == 4 ? (i & 1) * 4 + (i >> 1) : i;
+}
+
+// Eight codes (q4: one word; q8: two) -> eight values scale·code + bias of the type, chunk order.
+template <typename T, int BITS>
+__device__ __forceinline__ uint4 dequant8(uint32_t w0, uint32_t w1, T sc, T bi) {
+  uint32_t r[4];
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 s2 = __half2half2(sc), b2 = __half2half2(bi);
+    auto code = [](uint32_t x) { return *reinterpret_cast<__half2*>(&x); };
+    __half2 q[4];
+    if constexpr (BITS == 4) {
+      const __half2 k1024 = __float2half2_rn(1024.f), k16 = __float2half2_rn(0.0625f), k64 = __float2half2_rn(-64.f);
+      const uint32_t hi = w0 >> 8;
+      q[0] = __hsub2(code((w0 & 0x000F000Fu) | 0x64006400u), k1024);
+      q[1] = __hfma2(code((w0 & 0x00F000F0u) | 0x64006400u), k16, k64);
+      q[2] = __hsub2(code((hi & 0x000F000Fu) | 0x64006400u), k1024);
+      q[3] = __hfma2(code((hi & 0x00F000F0u) | 0x64006400u), k16, k64);
+    } else {
+      const __half2 k1024 = __float2half2_rn(1024.f);
+      q[0] = __hsub2(code(__byte_perm(w0, 0x64646464u, 0x4140)), k1024);
+      q[1] = __hsub2(code(__byte_perm(w0, 0x64646464u, 0x4342)), k1024);
+      q[2] = __hsub2(code(__byte_perm(w1, 0x64646464u, 0x4140)), k1024);
+      q[3] = __hsub2(code(__byte_perm(w1, 0x64646464u, 0x4342)), k1024);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 v = __hfma2(q[i], s2, b2);
+      r[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+  } else if constexpr (BITS == 4) {
+    const __nv_bfloat162 s2 = __bfloat162bfloat162(sc), b2 = __bfloat162bfloat162(bi);
+    const __nv_bfloat162 k128 = __float2bfloat162_rn(128.f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t x = ((w0 >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+      const __nv_bfloat162 v = __hfma2(__hsub2(*reinterpret_cast<__nv_bfloat162*>(&x), k128), s2, b2);
+      r[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+  } else {  // eight bits do not fit bf16's exponent trick: through fp32
+    const float s = to_f<T>(sc), b = to_f<T>(bi);
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = fmaf(s, (float)(((i < 4 ? w0 : w1) >> (8 * (i & 3))) & 255u), b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = pack2<T>(f[2 * i], f[2 * i + 1]);
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+// The output (or partial) row of a thread whose warp's unit has cleared drafted rows: O from tensor memory
+// plus Σ p_j·v_j over the cleared rows j that packed row pr (tree row t) sees, read from the cache. Their V
+// holds an infinity or NaN, so this runs for broken inputs only.
+template <typename T, int D, int BITS>
+__device__ __noinline__ void finish_cleared(const TreeArgs& a, int b, int g, const uint32_t (*bad)[8], int pr, int ctx,
+                                            float m_ref, float inv, uint32_t tcol, T* yrow, float* orow) {
+  const bool live = yrow || orow;
+  const int t = live ? pr % a.T : 0;
+  const T* q = static_cast<const T*>(a.q) + (((int64_t)b * a.HKV + g) * a.R + pr) * D;
+  const uint8_t* mask = a.mask ? a.mask + b * a.mask_b + (int64_t)t * a.T : nullptr;
+#pragma unroll 1
+  for (int cb = 0; cb < 2 * D / 32; ++cb) {
+    uint32_t ov[32];
+    tc::tmem_ld32(tcol + cb * 32, ov);
+    tc::tmem_ld_wait();
+    float o[32];
+#pragma unroll
+    for (int e = 0; e < 32; ++e) o[(e & ~7) + chunk_channel<BITS>(e & 7)] = __uint_as_float(ov[e]);
+    if (!live) continue;
+    for (int j = 0; j < a.T; ++j) {
+      const uint32_t w = bad[0][j >> 5] | bad[1][j >> 5] | bad[2][j >> 5] | bad[3][j >> 5];
+      if (!((w >> (j & 31)) & 1) || !(mask ? mask[j] != 0 : j <= t)) continue;
+      float s = 0.f, v[8];
+      for (int c8 = 0; c8 < D / 8; ++c8) {
+        load8<T, D, BITS>(a, 0, b, g, ctx + j, c8, v);
+        for (int e = 0; e < 8; ++e) s = fmaf(to_f<T>(q[c8 * 8 + e]), v[e], s);
+      }
+      const float p = exp2f(fmaf(s, a.scale_log2, m_ref == -INFINITY ? 0.f : -m_ref));
+      for (int c8 = 0; c8 < 4; ++c8) {
+        const int ch = cb * 4 + c8;
+        load8<T, D, BITS>(a, 1 + ch / (D / 8), b, g, ctx + j, ch % (D / 8), v);
+        for (int e = 0; e < 8; ++e) o[c8 * 8 + e] = fmaf(p, v[e], o[c8 * 8 + e]);
+      }
+    }
+    for (int e = 0; e < 32; ++e) {
+      if (yrow) yrow[cb * 32 + e] = from_f<T>(o[e] * inv);
+      else orow[cb * 32 + e] = o[e];
+    }
+  }
+}
+
+template <typename T, int D, int BITS>
+__global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const __grid_constant__ TcArgs ta) {
+  using Cfg = TcCfg<BITS>;
+  using Map = TcMap<D, BITS>;
+  constexpr int NS = Cfg::kStages;
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr uint32_t kColS = 0, kColO = 128, kCols = D == 128 ? 512 : 256;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const TreeArgs& a = ta.t;
+  const uint32_t sb = tc::smem_addr(smem);
+  const uint32_t bar = sb + Map::kBar;
+  const uint32_t q_full = bar;
+  auto k_full = [&](int s) { return bar + 8u * (1 + s); };
+  auto k_empty = [&](int s) { return bar + 8u * (1 + NS + s); };
+  auto v_full = [&](int s) { return bar + 8u * (1 + 2 * NS + s); };
+  auto v_empty = [&](int s) { return bar + 8u * (1 + 3 * NS + s); };
+  auto s_full = [&](int s) { return bar + 8u * (1 + 4 * NS + s); };
+  auto p_full = [&](int s) { return bar + 8u * (3 + 4 * NS + s); };
+  const uint32_t o_bar = bar + 8u * (5 + 4 * NS), drain = bar + 8u * (6 + 4 * NS);
+  auto raw_full = [&](int s) { return bar + 8u * (7 + 4 * NS + s); };
+  auto raw_empty = [&](int s) { return bar + 8u * (7 + 4 * NS + kRawMax + s); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Map::kBar + Map::kNumBars * 8);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  pdl_trigger();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < Map::kNumBars; ++i) {
+      int count = 1;
+      if (i == 0 || (i >= 3 + 4 * NS && i < 5 + 4 * NS)) count = 4;                              // q_full, p_full
+      if ((i >= 1 && i < 1 + NS) || (i >= 1 + 2 * NS && i < 1 + 3 * NS)) count = Cfg::kFill;     // k_full, v_full
+      if (i >= 7 + 4 * NS + kRawMax) count = Cfg::kFill;                                         // raw_empty
+      tc::mbar_init(bar + 8u * i, count);
+    }
+    *abort_flag = 0;
+    tc::mbar_fence_init();
+  }
+  if (warp == 1) {
+    tc::tmem_alloc(tc::smem_addr(tmem_slot), kCols);
+    tc::tmem_relinquish();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  Schedule sched(a);
+  Segment sg;
+  // Below, `it` counts this CTA's key tiles over all its segments: ring stages and barrier parities follow it.
+  if (warp == 0) {
+    if (lane == 0) {  // ---- copies ----
+      int it = 0, k_iss = 0, v_iss = 0;
+      bool ok = true;
+      while (ok && next_segment(a, sched, sg)) {
+        for (int kt = sg.t0; kt < sg.t1; ++kt, ++it) {
+          const int p0 = kt * kTK;
+          if (*abort_flag) { ok = false; break; }
+          if constexpr (BITS == 16) {
+            const int s = it % NS;
+            const uint32_t par = (it / NS - 1) & 1;
+            if (it >= NS && !tc::mbar_wait(k_empty(s), par)) { ok = false; break; }
+            const uint32_t kb = sb + Map::kK + s * Map::kKBytes;
+            tc::mbar_expect_tx(k_full(s), Map::kKBytes);
+#pragma unroll
+            for (int h = 0; h < Map::kHalves; ++h)
+              tc::tma_load_4d(kb + h * kTK * 128, &ta.tm[0], h * 128, p0, sg.g, sg.b, k_full(s));
+            k_iss = it + 1;
+            if (it >= NS && !tc::mbar_wait(v_empty(s), par)) { ok = false; break; }
+            const uint32_t vb = sb + Map::kV + s * Map::kVBytes;
+            tc::mbar_expect_tx(v_full(s), Map::kVBytes);
+#pragma unroll
+            for (int h = 0; h < 2 * Map::kHalves; ++h)
+              tc::tma_load_4d(vb + h * kTK * 128, &ta.tm[1 + h / Map::kHalves], (h % Map::kHalves) * 128, p0, sg.g, sg.b,
+                              v_full(s));
+            v_iss = it + 1;
+          } else {
+            const int s = it % ta.raw_stages;
+            if (it >= ta.raw_stages && !tc::mbar_wait(raw_empty(s), (it / ta.raw_stages - 1) & 1)) { ok = false; break; }
+            const int rows = min(kTK, a.cap - p0);
+            const int64_t row = ((int64_t)sg.b * a.HKV + sg.g) * a.cap + p0;
+            const uint32_t cb = rows * ta.code_bytes, gb = rows * ta.group_bytes;
+            uint32_t dst = sb + Map::kRaw + s * (3 * kTK * ta.code_bytes + 6 * kTK * ta.group_bytes);
+            tc::mbar_expect_tx(raw_full(s), 3 * cb + 6 * gb);
+#pragma unroll
+            for (int i = 0; i < 3; ++i, dst += kTK * ta.code_bytes)
+              tc::bulk_load(dst, static_cast<const char*>(a.kv[i]) + row * ta.code_bytes, cb, raw_full(s));
+#pragma unroll
+            for (int i = 0; i < 3; ++i, dst += 2 * kTK * ta.group_bytes) {
+              tc::bulk_load(dst, static_cast<const char*>(a.sc[i]) + row * ta.group_bytes, gb, raw_full(s));
+              tc::bulk_load(dst + kTK * ta.group_bytes, static_cast<const char*>(a.bi[i]) + row * ta.group_bytes, gb,
+                            raw_full(s));
+            }
+            k_iss = it + 1;
+          }
+        }
+      }
+      if (!ok) *abort_flag = 1;
+      // the copies issued last on each stage have landed before the CTA may exit
+      const int ring = BITS == 16 ? NS : ta.raw_stages;
+      for (int j = max(0, k_iss - ring); j < k_iss; ++j)
+        if (!tc::mbar_wait(BITS == 16 ? k_full(j % ring) : raw_full(j % ring), (j / ring) & 1)) *abort_flag = 1;
+      for (int j = max(0, v_iss - ring); j < v_iss; ++j)
+        if (!tc::mbar_wait(v_full(j % ring), (j / ring) & 1)) *abort_flag = 1;
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {  // ---- MMAs ----
+      constexpr uint32_t idesc_qk = tc::idesc_f16_f32(kTR, kTK, false, false, kBf16);
+      constexpr uint32_t idesc_pv = tc::idesc_f16_f32(kTR, 2 * D, true, false, kBf16);
+      auto issue_qk = [&](int it) -> bool {
+        const int s = it % NS;
+        if (!tc::mbar_wait(k_full(s), (it / NS) & 1)) return false;
+        tc::tc_fence_after();
+        const uint32_t kb = sb + Map::kK + s * Map::kKBytes;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          tc::mma_f16(tmem + kColS + 64 * (it & 1),
+                      tc::desc_kmajor_sw128(sb + Map::kQ + (kk >> 2) * kTR * 128 + (kk & 3) * 32),
+                      tc::desc_kmajor_sw128(kb + (kk >> 2) * kTK * 128 + (kk & 3) * 32), idesc_qk, kk > 0);
+        tc::mma_commit(s_full(it & 1));
+        tc::mma_commit(k_empty(s));
+        return true;
+      };
+      int it = 0, seg = 0;
+      bool ok = true;
+      for (; ok && next_segment(a, sched, sg); ++seg) {
+        ok = tc::mbar_wait(q_full, seg & 1) && issue_qk(it);
+        for (int kt = sg.t0; ok && kt < sg.t1; ++kt, ++it) {
+          if (*abort_flag || (kt + 1 < sg.t1 && !issue_qk(it + 1))) { ok = false; break; }
+          const int s = it % NS;
+          if (!tc::mbar_wait(p_full(it & 1), (it >> 1) & 1) || !tc::mbar_wait(v_full(s), (it / NS) & 1)) {
+            ok = false;
+            break;
+          }
+          tc::tc_fence_after();
+          const uint32_t pb = sb + Map::kP + (it & 1) * kTR * 128, vb = sb + Map::kV + s * Map::kVBytes;
+#pragma unroll
+          for (int kk = 0; kk < kTK / 16; ++kk)
+            tc::mma_f16(tmem + kColO, tc::desc_kmajor_sw128(pb + kk * 32),
+                        tc::desc_mnmajor_sw128(vb + kk * 2048, kTK * 128, 1024), idesc_pv, kt > sg.t0 || kk > 0);
+          tc::mma_commit(o_bar);
+          tc::mma_commit(v_empty(s));
+        }
+      }
+      if (!ok) *abort_flag = 1;
+      // every MMA this thread issued completes before tensor memory can be freed
+      tc::mma_commit(drain);
+      if (!tc::mbar_wait(drain, 0)) *abort_flag = 1;
+    }
+    __syncwarp();
+  } else if (warp < 6) {  // ---- softmax: one thread per query row ----
+    const int q = warp & 3;  // a warp reads tensor-memory lanes 32·(warp mod 4) ..
+    const int r = q * 32 + lane;
+    const uint32_t trow = tmem + ((uint32_t)(q * 32) << 16);
+    const float mult = fabsf(a.scale_log2);
+    auto load_q = [&](const Segment& g) {
+      const int pr = g.rt * kTR + r;
+      const T* src = static_cast<const T*>(a.q) + (((int64_t)g.b * a.HKV + g.g) * a.R + pr) * D;
+      const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;  // scale < 0: −q with |scale|
+#pragma unroll
+      for (int c8 = 0; c8 < D / 8; ++c8) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (pr < a.R) {
+          v = *reinterpret_cast<const uint4*>(src + c8 * 8);
+          if constexpr (BITS == 4)  // (0,1)(2,3)(4,5)(6,7) -> (0,4)(1,5)(2,6)(3,7)
+            v = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
+                           __byte_perm(v.y, v.w, 0x7632));
+          v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
+        }
+        *reinterpret_cast<uint4*>(smem + Map::kQ + (c8 >> 3) * kTR * 128 + r * 128 + (((c8 & 7) ^ (r & 7)) << 4)) = v;
+      }
+      tc::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(q_full);
+    };
+    bool alive = true;
+    int it = 0, seg = 0;
+    Segment nx;
+    bool more = next_segment(a, sched, nx);
+    if (more) load_q(nx);
+    while (more) {
+      sg = nx;
+      const int pr = sg.rt * kTR + r;
+      const bool live = pr < a.R;
+      const bool work = sg.rt * kTR + q * 32 < a.R;  // this warp has a row
+      const int t = live ? pr % a.T : 0;
+      const int ctx = sg.n - a.T;
+      uint32_t(*bad)[8] = reinterpret_cast<uint32_t(*)[8]>(smem + Map::kBad + (seg & 1) * 4 * 8 * 4);
+      if (lane < 8) bad[q][lane] = 0;
+      __syncwarp();
+      float m_ref = -INFINITY, l = 0.f;
+      for (int kt = sg.t0; alive && kt < sg.t1; ++kt, ++it) {
+        const int s = it & 1, p0 = kt * kTK;
+        const bool tail = p0 + kTK > ctx;  // drafted rows or the cache's end in this tile
+        uint64_t vis = 0;
+        if (tail && live) vis = visible<kTK>(a, sg.b, t, sg.n, p0);
+        const bool got = tc::mbar_wait(s_full(s), (it >> 1) & 1);
+        if (__any_sync(0xffffffffu, !got || *abort_flag)) {
+          alive = false;
+          break;
+        }
+        tc::tc_fence_after();
+        uint32_t pk[32];
+        bool need = false;
+        float factor = 1.f;
+        if (work) {
+          uint32_t sv[2][32];
+          tc::tmem_ld32(trow + kColS + 64 * s, sv[0]);
+          tc::tmem_ld32(trow + kColS + 64 * s + 32, sv[1]);
+          tc::tmem_ld_wait();
+          float mul = mult, m_tile = -INFINITY;
+          if (tail) {
+            mul = 1.f;
+#pragma unroll
+            for (int c = 0; c < 64; ++c) {
+              const float x = __uint_as_float(sv[c >> 5][c & 31]) * mult;
+              sv[c >> 5][c & 31] = __float_as_uint((vis >> c) & 1 ? x : -INFINITY);
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < 64; ++c) m_tile = fmaxf(m_tile, __uint_as_float(sv[c >> 5][c & 31]));
+          m_tile = m_tile == -INFINITY ? -INFINITY : m_tile * mul;
+          need = m_tile > m_ref + 8.f;
+          if (need) {
+            factor = ex2(m_ref - m_tile);  // 0 at the first visible key
+            m_ref = m_tile;
+          }
+          l *= factor;
+          const float mb = m_ref == -INFINITY ? 0.f : m_ref;
+          float ps[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 64; c += 2) {
+            const float e0 = ex2(fmaf(__uint_as_float(sv[c >> 5][c & 31]), mul, -mb));
+            const float e1 = ex2(fmaf(__uint_as_float(sv[c >> 5][(c & 31) + 1]), mul, -mb));
+            ps[(c >> 1) & 3] += e0 + e1;
+            pk[c >> 1] = pack2<T>(e0, e1);  // P in the type: one rounding of each weight
+          }
+          l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+        }
+        if (tail) {  // clear the V rows a zero weight may not meet
+          const int st = it % NS;
+          const bool vok = tc::mbar_wait(v_full(st), (it / NS) & 1);
+          if (__any_sync(0xffffffffu, !vok)) {
+            alive = false;
+            break;
+          }
+          const int vr = q * 16 + (lane >> 1), pos = p0 + vr;
+          bool clear = pos >= sg.n;
+          uint8_t* vrow = smem + Map::kV + st * Map::kVBytes + (lane & 1) * Map::kHalves * kTK * 128 + vr * 128;
+          if (!clear && pos >= ctx) {
+            bool nf = false;
+#pragma unroll
+            for (int h = 0; h < Map::kHalves; ++h)
+#pragma unroll
+              for (int c = 0; c < 8; ++c) {
+                const uint4 v = *reinterpret_cast<const uint4*>(vrow + h * kTK * 128 + c * 16);
+                nf |= nonfinite2<T>(v.x) | nonfinite2<T>(v.y) | nonfinite2<T>(v.z) | nonfinite2<T>(v.w);
+              }
+            clear = nf;
+          }
+          clear |= __shfl_xor_sync(0xffffffffu, clear, 1);
+          if (clear) {
+#pragma unroll
+            for (int h = 0; h < Map::kHalves; ++h)
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                *reinterpret_cast<uint4*>(vrow + h * kTK * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+            if (pos < sg.n && (lane & 1) == 0) atomicOr(&bad[q][(pos - ctx) >> 5], 1u << ((pos - ctx) & 31));
+          }
+        }
+        // O and the P buffer are free once the last P·V has completed
+        if (kt > sg.t0) {
+          const bool done = tc::mbar_wait(o_bar, (it - 1) & 1);
+          if (__any_sync(0xffffffffu, !done)) {
+            alive = false;
+            break;
+          }
+          tc::tc_fence_after();
+          if (__any_sync(0xffffffffu, need)) {
+#pragma unroll 1
+            for (int cb = 0; cb < 2 * D / 32; ++cb) {
+              uint32_t ov[32];
+              tc::tmem_ld32(trow + kColO + cb * 32, ov);
+              tc::tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * factor);
+              tc::tmem_st32(trow + kColO + cb * 32, ov);
+            }
+            tc::tmem_st_wait();
+          }
+        }
+        if (work) {
+          uint8_t* prow = smem + Map::kP + s * kTR * 128 + r * 128;
+#pragma unroll
+          for (int c8 = 0; c8 < 8; ++c8)
+            *reinterpret_cast<uint4*>(prow + ((c8 ^ (r & 7)) << 4)) =
+                make_uint4(pk[4 * c8], pk[4 * c8 + 1], pk[4 * c8 + 2], pk[4 * c8 + 3]);
+        }
+        tc::fence_proxy_async_smem();
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(p_full(s));
+      }
+      more = next_segment(a, sched, nx);
+      // the segment's last S is complete: its Q is free, and the next one's first product can start
+      if (more && alive) load_q(nx);
+      if (alive) alive = __all_sync(0xffffffffu, tc::mbar_wait(o_bar, (it - 1) & 1));
+      if (!alive) *abort_flag = 1;
+      tc::tc_fence_after();
+      if (work) {
+        // Through this warp's 4 KB of the P buffer of the next tile's other half: the last P·V has read it.
+        const float inv = !alive ? NAN : l == 0.f ? 0.f : 1.f / l;
+        uint8_t* stage = smem + Map::kP + q * 32 * 128;
+        const int64_t row0 = ((int64_t)sg.b * a.HKV + sg.g) * a.R + sg.rt * kTR + q * 32;  // first of the warp's rows
+        const int rows = min(32, a.R - (sg.rt * kTR + q * 32));
+        uint32_t any_bad = 0;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) any_bad |= bad[0][w] | bad[1][w] | bad[2][w] | bad[3][w];
+        if (sg.slot >= 0 && live) {
+          float* ml = a.part_ml + ((int64_t)sg.slot * a.slot_rows + r) * 2;
+          ml[0] = m_ref;
+          ml[1] = alive ? l : NAN;
+        }
+        if (any_bad && alive) {  // any_bad is the same in the whole CTA
+          T* yrow = live && sg.slot < 0 ? static_cast<T*>(a.y) + (row0 + lane) * 2 * D : nullptr;
+          float* orow = live && sg.slot >= 0 ? a.part_o + ((int64_t)sg.slot * a.slot_rows + r) * 2 * D : nullptr;
+          finish_cleared<T, D, BITS>(a, sg.b, sg.g, bad, live ? pr : 0, ctx, m_ref, inv, trow + kColO, yrow, orow);
+        } else
+#pragma unroll 1
+        for (int cb = 0; cb < 2 * D / 32; ++cb) {
+          uint32_t ov[32];
+          tc::tmem_ld32(trow + kColO + cb * 32, ov);
+          tc::tmem_ld_wait();
+          float o[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[(e & ~7) + chunk_channel<BITS>(e & 7)] = alive ? __uint_as_float(ov[e]) : NAN;
+          if (sg.slot < 0) {  // 32 rows × 64 bytes
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint4 v;
+              v.x = pack2<T>(o[8 * c] * inv, o[8 * c + 1] * inv);
+              v.y = pack2<T>(o[8 * c + 2] * inv, o[8 * c + 3] * inv);
+              v.z = pack2<T>(o[8 * c + 4] * inv, o[8 * c + 5] * inv);
+              v.w = pack2<T>(o[8 * c + 6] * inv, o[8 * c + 7] * inv);
+              *reinterpret_cast<uint4*>(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = v;
+            }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int rr = i * 8 + (lane >> 2), c = lane & 3;
+              const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 64 + ((c ^ ((rr >> 1) & 3)) << 4));
+              if (rr < rows)
+                *reinterpret_cast<uint4*>(static_cast<T*>(a.y) + (row0 + rr) * 2 * D + cb * 32 + c * 8) = v;
+            }
+          } else {  // 32 rows × 128 bytes
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              *reinterpret_cast<float4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+                  make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int rr = i * 4 + (lane >> 3), c = lane & 7;
+              const float4 v = *reinterpret_cast<const float4*>(stage + rr * 128 + ((c ^ (rr & 7)) << 4));
+              if (rr < rows)
+                *reinterpret_cast<float4*>(a.part_o + ((int64_t)sg.slot * a.slot_rows + q * 32 + rr) * 2 * D + cb * 32 +
+                                           c * 4) = v;
+            }
+          }
+          __syncwarp();
+        }
+      }
+      ++seg;
+    }
+  } else if constexpr (BITS != 16) {  // ---- operand tiles from packed rows ----
+    const int tid = threadIdx.x - 192;
+    constexpr int kUnits = kTK * D / 32;  // 32 channels of one row
+    auto fill = [&](const uint8_t* codes, const uint8_t* scales, uint8_t* tile) {
+      for (int u = tid; u < kUnits; u += 256) {
+        const int row = u / (D / 32), c32 = u % (D / 32);
+        // the four chunks' order differs between a row's halves so that eight lanes write to eight bank groups
+        const int flip = D == 128 ? (c32 >> 1) << 1 : 0;
+        uint32_t w[BITS];
+        const uint4* src = reinterpret_cast<const uint4*>(codes + row * ta.code_bytes + c32 * BITS * 4);
+#pragma unroll
+        for (int i = 0; i < BITS / 4; ++i) *reinterpret_cast<uint4*>(w + 4 * i) = src[i];
+        const T* sc = reinterpret_cast<const T*>(scales + row * ta.group_bytes);
+        const T* bi = reinterpret_cast<const T*>(scales + kTK * ta.group_bytes + row * ta.group_bytes);
+        T s = sc[c32 * 32 / a.gs], b = bi[c32 * 32 / a.gs];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int kx = k ^ flip;
+          uint32_t w0, w1 = 0;
+          if constexpr (BITS == 4) {
+            w0 = flip ? w[k ^ 2] : w[k];
+          } else {
+            w0 = flip ? w[2 * (k ^ 2)] : w[2 * k];
+            w1 = flip ? w[2 * (k ^ 2) + 1] : w[2 * k + 1];
+          }
+          const int c8 = c32 * 4 + kx;
+          if (a.gs < 32) s = sc[c8 * 8 / a.gs], b = bi[c8 * 8 / a.gs];
+          *reinterpret_cast<uint4*>(tile + (c8 >> 3) * kTK * 128 + row * 128 + (((c8 & 7) ^ (row & 7)) << 4)) =
+              dequant8<T, BITS>(w0, w1, s, b);
+        }
+      }
+      tc::fence_proxy_async_smem();
+      __syncwarp();
+    };
+    int it = 0;
+    bool alive = true;
+    while (alive && next_segment(a, sched, sg)) {
+      for (int kt = sg.t0; kt < sg.t1; ++kt, ++it) {
+        const int rs = it % ta.raw_stages, s = it % NS;
+        const uint32_t par = (it / NS - 1) & 1;
+        bool ok = tc::mbar_wait(raw_full(rs), (it / ta.raw_stages) & 1) && (it < NS || tc::mbar_wait(k_empty(s), par));
+        if (__any_sync(0xffffffffu, !ok || *abort_flag)) { alive = false; break; }
+        const uint8_t* raw = smem + Map::kRaw + rs * (3 * kTK * ta.code_bytes + 6 * kTK * ta.group_bytes);
+        const uint8_t* rsc = raw + 3 * kTK * ta.code_bytes;
+        fill(raw, rsc, smem + Map::kK + s * Map::kKBytes);
+        if (lane == 0) tc::mbar_arrive(k_full(s));
+        ok = it < NS || tc::mbar_wait(v_empty(s), par);
+        if (__any_sync(0xffffffffu, !ok)) { alive = false; break; }
+        uint8_t* vt = smem + Map::kV + s * Map::kVBytes;
+        fill(raw + kTK * ta.code_bytes, rsc + 2 * kTK * ta.group_bytes, vt);
+        fill(raw + 2 * kTK * ta.code_bytes, rsc + 4 * kTK * ta.group_bytes, vt + Map::kKBytes);
+        if (lane == 0) {
+          tc::mbar_arrive(v_full(s));
+          tc::mbar_arrive(raw_empty(rs));
+        }
+      }
+    }
+    if (!alive) *abort_flag = 1;
+  }
+
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tmem, kCols);
+  }
+  if (threadIdx.x == 0 && *abort_flag && a.err) atomicExch(a.err, 1);
 }
 
 // ---- join of the cut units' partials -----------------------------------------------------------------
@@ -321,7 +928,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__
   auto lo = [&](int64_t i) { return i * total / grid; };
   const int64_t i0 = ((s + 1) * grid - 1) / total, i1 = (e * grid - 1) / total;  // CTAs of tiles s and e − 1
   if (i0 == i1) return;  // written by its CTA
-  auto slot_row = [&](int64_t i) { return (2 * i + (lo(i) >= s ? 0 : 1)) * a.tile_rows + r; };
+  auto slot_row = [&](int64_t i) { return (2 * i + (lo(i) >= s ? 0 : 1)) * a.slot_rows + r; };
   float M = -INFINITY;
   for (int64_t i = i0; i <= i1; ++i)
     if (lo(i) < lo(i + 1)) M = fmaxf(M, a.part_ml[slot_row(i) * 2]);
@@ -358,11 +965,32 @@ int sm_count() {
   return n;
 }
 
-// CTAs of the attention launch: as many as run at once, at most one per key tile of the longest lengths.
-int64_t grid_of(const TreeArgs& a, int64_t ctas, int64_t len_bound) {
-  const int64_t nt = ceil_div(len_bound < 1 ? 1 : len_bound, a.tile_keys);
-  const int64_t all = nt * a.B * a.HKV * a.row_tiles;
-  return all < ctas ? all : ctas;
+constexpr int64_t kMaxTreeRows = 256;
+
+// Which kernel serves a call, and its launch shape.
+struct Plan {
+  bool tc;
+  int tile_rows, tile_keys, row_tiles, slot_rows;
+  int64_t tiles;  // key tiles of all units at the longest lengths
+  int64_t grid;   // at most the CTAs that run at once, and one per tile
+  size_t ml_offset, bytes;
+};
+
+// The tensor-core form takes 16-bit types; packed rows need tiles that start on 16-byte boundaries in the
+// scales too (any capacity that is a multiple of 8 does). The rest runs on the CUDA cores.
+Plan make_plan(int dtype, int bits, int gs, int64_t B, int64_t HKV, int64_t R, int64_t D, int64_t cap, int64_t len_bound) {
+  Plan p{};
+  p.tc = dtype != MOTIF_F32 && (bits == 16 || (cap * (D / gs)) % 8 == 0);
+  p.tile_rows = p.tc ? kTR : kSR;
+  p.tile_keys = p.tc ? kTK : kSK;
+  p.row_tiles = (int)ceil_div(R, p.tile_rows);
+  p.slot_rows = (int)(R < p.tile_rows ? R : p.tile_rows);
+  const int64_t ctas = (p.tc ? 1 : 2) * (int64_t)sm_count();
+  p.tiles = ceil_div(len_bound < 1 ? 1 : len_bound, p.tile_keys) * B * HKV * p.row_tiles;
+  p.grid = p.tiles < ctas ? p.tiles : ctas;
+  p.ml_offset = sizeof(float) * 2 * (size_t)p.grid * p.slot_rows * 2 * (size_t)D;
+  p.bytes = p.ml_offset + sizeof(float) * 2 * (size_t)p.grid * p.slot_rows * 2;
+  return p;
 }
 
 template <typename T, int D>
@@ -391,17 +1019,40 @@ int launch_simt(TreeArgs& a, int64_t grid, cudaStream_t st) {
   return rc ? rc : launch_merge<T, D>(a, grid, st);
 }
 
-constexpr int64_t kMaxTreeRows = 256;
+template <typename T, int D, int BITS>
+int launch_tc(const TreeArgs& a, int64_t grid, cudaStream_t st) {
+  using Map = TcMap<D, BITS>;
+  TcArgs ta{};
+  ta.t = a;
+  int smem = 1024 + Map::kRaw;
+  if constexpr (BITS == 16) {
+    const uint64_t dims[3] = {(uint64_t)a.cap, (uint64_t)a.HKV, (uint64_t)a.B};
+    const uint64_t strides[3] = {(uint64_t)a.sr * 2, (uint64_t)a.sh * 2, (uint64_t)a.sb * 2};
+    for (int i = 0; i < 3; ++i)
+      if (!encode_tma_heads(&ta.tm[i], a.kv[i], D * 2, dims, strides, 128, kTK))
+        return fail(MOTIF_ERR_CUDA, "sdpa_dual_v_tree: tensor map encoding failed");
+  } else {
+    ta.code_bytes = D * BITS / 8;
+    ta.group_bytes = D / a.gs * 2;
+    const int raw = 3 * kTK * ta.code_bytes + 6 * kTK * ta.group_bytes;
+    const int room = 227 * 1024 - smem;
+    ta.raw_stages = room / raw < kRawMax ? room / raw : kRawMax;
+    if (ta.raw_stages < 1) return fail(MOTIF_ERR_BAD_CONTRACT, "sdpa_dual_v_tree: group_size %d too small", a.gs);
+    smem += ta.raw_stages * raw;
+  }
+  auto kern = tree_tc_kernel<T, D, BITS>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return fail(MOTIF_ERR_CUDA, "sdpa_dual_v_tree: smem attribute: %s", cudaGetErrorString(e));
+  kern<<<(unsigned)grid, TcCfg<BITS>::kThreads, smem, st>>>(ta);
+  const int rc = check_launch("sdpa_dual_v_tree");
+  return rc ? rc : launch_merge<T, D>(a, grid, st);
+}
 
-struct Plan {
-  int tile_rows, tile_keys;
-  int64_t ctas;  // CTAs that run at once
-};
-
-Plan plan_of() { return Plan{kSR, kSK, 2 * (int64_t)sm_count()}; }
-
-size_t workspace_of(const Plan& p, int64_t D) {
-  return sizeof(float) * 2 * (size_t)p.ctas * (size_t)p.tile_rows * (size_t)(2 * D + 2);
+template <typename T, int D, int BITS>
+int launch(TreeArgs& a, const Plan& p, cudaStream_t st) {
+  if constexpr (!std::is_same<T, float>::value)
+    if (p.tc) return launch_tc<T, D, BITS>(a, p.grid, st);
+  return launch_simt<T, D, BITS>(a, p.grid, st);
 }
 
 }  // namespace
@@ -411,8 +1062,13 @@ using namespace motif;
 
 extern "C" {
 
-size_t motif_sdpa_dual_v_tree_workspace_bytes(int64_t head_dim) {
-  return workspace_of(plan_of(), head_dim);
+size_t motif_sdpa_dual_v_tree_workspace_bytes(int dtype, int bits, int group_size, int64_t batch, int64_t h_q,
+                                              int64_t h_kv, int64_t tree_rows, int64_t kv_cap, int64_t head_dim,
+                                              int64_t kv_len_bound) {
+  if (batch < 1 || h_q < 1 || h_kv < 1 || tree_rows < 1 || kv_cap < 1 || head_dim < 1 || group_size < 1 ||
+      head_dim < group_size)
+    return 0;
+  return make_plan(dtype, bits, group_size, batch, h_kv, h_q / h_kv * tree_rows, head_dim, kv_cap, kv_len_bound).bytes;
 }
 
 int motif_sdpa_dual_v_tree(int dtype, int bits, int group_size, const void* q, const motif_tree_kv* kv,
@@ -448,8 +1104,7 @@ int motif_sdpa_dual_v_tree(int dtype, int bits, int group_size, const void* q, c
     al |= reinterpret_cast<uintptr_t>(kv->data[i]);
     if (bits != 16) {
       MOTIF_REQUIRE(kv->scales[i] && kv->biases[i], MOTIF_ERR_NULL, "sdpa_dual_v_tree: slot %d scales/biases null", i);
-      MOTIF_REQUIRE((reinterpret_cast<uintptr_t>(kv->scales[i]) | reinterpret_cast<uintptr_t>(kv->biases[i])) % esz == 0,
-                    MOTIF_ERR_BAD_CONTRACT, "sdpa_dual_v_tree: misaligned scales/biases");
+      al |= reinterpret_cast<uintptr_t>(kv->scales[i]) | reinterpret_cast<uintptr_t>(kv->biases[i]);
     }
   }
   MOTIF_REQUIRE(al % 16 == 0, MOTIF_ERR_BAD_CONTRACT, "sdpa_dual_v_tree: operands must be 16-byte aligned");
@@ -487,27 +1142,30 @@ int motif_sdpa_dual_v_tree(int dtype, int bits, int group_size, const void* q, c
   a.cap = (int)kv_cap;
   a.gs = group_size;
   a.scale_log2 = scale * kLog2e;
-  const Plan p = plan_of();
+  const Plan p = make_plan(dtype, bits, bits == 16 ? 64 : group_size, batch, h_kv, a.R, head_dim, kv_cap,
+                           kv_len_dev ? kv_cap : kv_len);
   a.tile_rows = p.tile_rows;
   a.tile_keys = p.tile_keys;
-  a.row_tiles = (int)ceil_div(a.R, p.tile_rows);
-  MOTIF_REQUIRE(workspace && workspace_bytes >= workspace_of(p, head_dim), MOTIF_ERR_WORKSPACE,
-                "sdpa_dual_v_tree: workspace of %zu bytes, needs %zu", workspace_bytes, workspace_of(p, head_dim));
+  a.row_tiles = p.row_tiles;
+  a.slot_rows = p.slot_rows;
+  MOTIF_REQUIRE(p.tiles < (1ll << 31) - 1, MOTIF_ERR_BAD_SHAPE, "sdpa_dual_v_tree: %lld key tiles in one call",
+                (long long)p.tiles);
+  MOTIF_REQUIRE(workspace && workspace_bytes >= p.bytes, MOTIF_ERR_WORKSPACE,
+                "sdpa_dual_v_tree: workspace of %zu bytes, needs %zu", workspace_bytes, p.bytes);
   MOTIF_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, MOTIF_ERR_BAD_CONTRACT,
                 "sdpa_dual_v_tree: workspace must be 16-byte aligned");
   a.part_o = static_cast<float*>(workspace);
-  a.part_ml = a.part_o + 2 * p.ctas * p.tile_rows * 2 * head_dim;
-  const int64_t grid = grid_of(a, p.ctas, kv_len_dev ? kv_cap : kv_len);
+  a.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.ml_offset);
   cudaStream_t st = as_stream(stream);
   MOTIF_DISPATCH_FLOAT(dtype, T, {
     if (head_dim == 64) {
-      if (bits == 16) return launch_simt<T, 64, 16>(a, grid, st);
-      if (bits == 4) return launch_simt<T, 64, 4>(a, grid, st);
-      return launch_simt<T, 64, 8>(a, grid, st);
+      if (bits == 16) return launch<T, 64, 16>(a, p, st);
+      if (bits == 4) return launch<T, 64, 4>(a, p, st);
+      return launch<T, 64, 8>(a, p, st);
     }
-    if (bits == 16) return launch_simt<T, 128, 16>(a, grid, st);
-    if (bits == 4) return launch_simt<T, 128, 4>(a, grid, st);
-    return launch_simt<T, 128, 8>(a, grid, st);
+    if (bits == 16) return launch<T, 128, 16>(a, p, st);
+    if (bits == 4) return launch<T, 128, 4>(a, p, st);
+    return launch<T, 128, 8>(a, p, st);
   });
   return MOTIF_OK;
 }
