@@ -291,11 +291,15 @@ __global__ void __launch_bounds__(kSThreads, 2) tree_simt_kernel(const __grid_co
 //   warp 0       TMA: K and V tiles straight from the cache into rings of kStages (16-bit rows), or the
 //                packed rows, scales and biases into a ring of raw tiles;
 //   warp 1       one lane issues the MMAs, S one tile ahead within a segment;
-//   warps 2..5   a thread is a query row: loads Q, takes S from tensor memory, keeps the running maximum
-//                and sum, writes P in the type; O is rescaled in tensor memory only when a row's maximum
-//                grew by more than 2^8 (weights stay ≤ 256, and the result is exact). Warps without a row
-//                only keep the barriers.
-//   warps 6..13  (packed) rebuild K and V tiles from the codes with packed 16-bit arithmetic: the code is
+//   warps 2..9   two softmax groups of four warps that take the tiles in turn (one warp alone on a
+//                scheduler waits out every latency of its 64-column row: tensor-memory reads, the maximum,
+//                the exponentials). A thread is a query row: it takes S from tensor memory and writes P in
+//                the type. The groups share the row's reference maximum, handed from tile to tile; it is
+//                raised, and O rescaled in tensor memory, only when a row's maximum grew by more than 2^8
+//                (weights stay ≤ 256, and the result is exact). Each group sums its own tiles' weights; at
+//                the end group A writes the V1 half of the rows and group B the V2 half. Warps without a
+//                row only keep the barriers.
+//   warps 10..15 (packed) rebuild K and V tiles from the codes with packed 16-bit arithmetic: the code is
 //                exact in the type (exponent trick), scale·code + bias one fused rounding.
 // Where the tile holds drafted rows or the cache's end, the softmax warps clear V rows that no query may
 // use (rows ≥ n, whatever the buffer holds) and drafted rows with a non-finite value: a zero weight times
@@ -308,8 +312,8 @@ constexpr int kTR = 128, kTK = 64;
 template <int BITS>
 struct TcCfg {
   static constexpr int kStages = BITS == 16 ? 3 : 2;  // K/V operand tiles
-  static constexpr int kThreads = BITS == 16 ? 192 : 448;
-  static constexpr int kFill = BITS == 16 ? 1 : 8;  // arrivals that fill a K or V tile
+  static constexpr int kThreads = BITS == 16 ? 320 : 512;
+  static constexpr int kFill = BITS == 16 ? 1 : 6;  // arrivals that fill a K or V tile
 };
 constexpr int kRawMax = 4;
 
@@ -317,6 +321,11 @@ struct TcArgs {
   TreeArgs t;
   CUtensorMap tm[3];  // k, v1, v2 rows
   int raw_stages, code_bytes, group_bytes;  // packed: ring depth, bytes of a row's codes and of its scales
+};
+
+struct Cleared {
+  int seg;           // the segment the bits belong to
+  uint32_t bits[8];  // tree rows
 };
 
 template <int D, int BITS>
@@ -329,10 +338,25 @@ struct TcMap {  // shared memory, bytes from a 1024-byte boundary
   static constexpr int kVBytes = 2 * kKBytes;
   static constexpr int kP = kV + TcCfg<BITS>::kStages * kVBytes;
   static constexpr int kBar = kP + 2 * kTR * 128;
-  static constexpr int kNumBars = 1 + 4 * TcCfg<BITS>::kStages + 4 + 2 + 2 * kRawMax;
-  static constexpr int kBad = kBar + kNumBars * 8 + 16;  // [2 segments][4 warps][8 words]: drafted rows cleared
-  static constexpr int kRaw = (kBad + 2 * 4 * 8 * 4 + 127) / 128 * 128;
+  static constexpr int kNumBars = 1 + 4 * TcCfg<BITS>::kStages + 4 + 3 + 2 * kRawMax + 12;
+  static constexpr int kState = kBar + kNumBars * 8 + 16;  // [128] reference maxima, [2][128] sums of the groups
+  static constexpr int kBad = kState + 3 * kTR * 4;        // drafted rows cleared: [2 segments][8 warps] Cleared
+  static constexpr int kRaw = (kBad + 2 * 8 * (int)sizeof(Cleared) + 127) / 128 * 128;
 };
+
+// Bounded mbarrier wait: about half a second of polls, far above any pipeline stage.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+  for (int i = 0; i < (1 << 16); ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.b32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+  }
+  return false;
+}
 
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b);
@@ -412,43 +436,37 @@ __device__ __forceinline__ uint4 dequant8(uint32_t w0, uint32_t w1, T sc, T bi) 
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
-// The output (or partial) row of a thread whose warp's unit has cleared drafted rows: O from tensor memory
-// plus Σ p_j·v_j over the cleared rows j that packed row pr (tree row t) sees, read from the cache. Their V
-// holds an infinity or NaN, so this runs for broken inputs only.
+// Adds Σ p_j·v_j over the cleared drafted rows j that packed row pr (tree row t) sees to half `grp` of its output
+// (yrow, normalised by inv) or partial (orow), read from the cache. Their V holds an infinity or NaN, so this
+// runs for broken inputs only; the finite channels of such an output row are rounded once more per row added.
 template <typename T, int D, int BITS>
-__device__ __noinline__ void finish_cleared(const TreeArgs& a, int b, int g, const uint32_t (*bad)[8], int pr, int ctx,
-                                            float m_ref, float inv, uint32_t tcol, T* yrow, float* orow) {
-  const bool live = yrow || orow;
-  const int t = live ? pr % a.T : 0;
+__device__ __forceinline__ void add_cleared(const TreeArgs& a, int b, int g, const Cleared* bad, int seg, int pr, int t,
+                                            int ctx, float m_ref, float inv, int grp, T* yrow, float* orow) {
   const T* q = static_cast<const T*>(a.q) + (((int64_t)b * a.HKV + g) * a.R + pr) * D;
-  const uint8_t* mask = a.mask ? a.mask + b * a.mask_b + (int64_t)t * a.T : nullptr;
 #pragma unroll 1
-  for (int cb = 0; cb < 2 * D / 32; ++cb) {
-    uint32_t ov[32];
-    tc::tmem_ld32(tcol + cb * 32, ov);
-    tc::tmem_ld_wait();
-    float o[32];
+  for (int j = 0; j < a.T; ++j) {
+    uint32_t w = 0;
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) w |= bad[i].seg == seg ? bad[i].bits[j >> 5] : 0u;
+    if (!((w >> (j & 31)) & 1)) continue;
+    if (!(a.mask ? a.mask[b * a.mask_b + (int64_t)t * a.T + j] != 0 : j <= t)) continue;
+    float s = 0.f, v[8];
+#pragma unroll 1
+    for (int c8 = 0; c8 < D / 8; ++c8) {
+      load8<T, D, BITS>(a, 0, b, g, ctx + j, c8, v);
 #pragma unroll
-    for (int e = 0; e < 32; ++e) o[(e & ~7) + chunk_channel<BITS>(e & 7)] = __uint_as_float(ov[e]);
-    if (!live) continue;
-    for (int j = 0; j < a.T; ++j) {
-      const uint32_t w = bad[0][j >> 5] | bad[1][j >> 5] | bad[2][j >> 5] | bad[3][j >> 5];
-      if (!((w >> (j & 31)) & 1) || !(mask ? mask[j] != 0 : j <= t)) continue;
-      float s = 0.f, v[8];
-      for (int c8 = 0; c8 < D / 8; ++c8) {
-        load8<T, D, BITS>(a, 0, b, g, ctx + j, c8, v);
-        for (int e = 0; e < 8; ++e) s = fmaf(to_f<T>(q[c8 * 8 + e]), v[e], s);
-      }
-      const float p = exp2f(fmaf(s, a.scale_log2, m_ref == -INFINITY ? 0.f : -m_ref));
-      for (int c8 = 0; c8 < 4; ++c8) {
-        const int ch = cb * 4 + c8;
-        load8<T, D, BITS>(a, 1 + ch / (D / 8), b, g, ctx + j, ch % (D / 8), v);
-        for (int e = 0; e < 8; ++e) o[c8 * 8 + e] = fmaf(p, v[e], o[c8 * 8 + e]);
-      }
+      for (int e = 0; e < 8; ++e) s = fmaf(to_f<T>(q[c8 * 8 + e]), v[e], s);
     }
-    for (int e = 0; e < 32; ++e) {
-      if (yrow) yrow[cb * 32 + e] = from_f<T>(o[e] * inv);
-      else orow[cb * 32 + e] = o[e];
+    const float p = exp2f(fmaf(s, a.scale_log2, m_ref == -INFINITY ? 0.f : -m_ref));
+#pragma unroll 1
+    for (int c8 = 0; c8 < D / 8; ++c8) {
+      load8<T, D, BITS>(a, 1 + grp, b, g, ctx + j, c8, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = grp * D + c8 * 8 + e;
+        if (yrow) yrow[c] = from_f<T>(fmaf(p * inv, v[e], to_f<T>(yrow[c])));
+        else orow[c] = fmaf(p, v[e], orow[c]);
+      }
     }
   }
 }
@@ -472,9 +490,12 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
   auto v_empty = [&](int s) { return bar + 8u * (1 + 3 * NS + s); };
   auto s_full = [&](int s) { return bar + 8u * (1 + 4 * NS + s); };
   auto p_full = [&](int s) { return bar + 8u * (3 + 4 * NS + s); };
-  const uint32_t o_bar = bar + 8u * (5 + 4 * NS), drain = bar + 8u * (6 + 4 * NS);
-  auto raw_full = [&](int s) { return bar + 8u * (7 + 4 * NS + s); };
-  auto raw_empty = [&](int s) { return bar + 8u * (7 + 4 * NS + kRawMax + s); };
+  auto o_done = [&](int s) { return bar + 8u * (5 + 4 * NS + s); };  // P·V of tiles of parity s
+  const uint32_t drain = bar + 8u * (7 + 4 * NS);
+  auto raw_full = [&](int s) { return bar + 8u * (8 + 4 * NS + s); };
+  auto raw_empty = [&](int s) { return bar + 8u * (8 + 4 * NS + kRawMax + s); };
+  auto m_next = [&](int g, int q) { return bar + 8u * (8 + 4 * NS + 2 * kRawMax + 4 * g + q); };  // maxima handed on by group g
+  auto l_both = [&](int q) { return bar + 8u * (16 + 4 * NS + 2 * kRawMax + q); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Map::kBar + Map::kNumBars * 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -483,12 +504,15 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
   if (threadIdx.x == 0) {
     for (int i = 0; i < Map::kNumBars; ++i) {
       int count = 1;
-      if (i == 0 || (i >= 3 + 4 * NS && i < 5 + 4 * NS)) count = 4;                              // q_full, p_full
-      if ((i >= 1 && i < 1 + NS) || (i >= 1 + 2 * NS && i < 1 + 3 * NS)) count = Cfg::kFill;     // k_full, v_full
-      if (i >= 7 + 4 * NS + kRawMax) count = Cfg::kFill;                                         // raw_empty
+      if (i == 0) count = 8;                                                                  // q_full
+      if ((i >= 1 && i < 1 + NS) || (i >= 1 + 2 * NS && i < 1 + 3 * NS)) count = Cfg::kFill;  // k_full, v_full
+      if (i >= 3 + 4 * NS && i < 5 + 4 * NS) count = 4;                                       // p_full
+      if (i >= 8 + 4 * NS + kRawMax && i < 8 + 4 * NS + 2 * kRawMax) count = Cfg::kFill;      // raw_empty
+      if (i >= 16 + 4 * NS + 2 * kRawMax) count = 2;                                          // l_both
       tc::mbar_init(bar + 8u * i, count);
     }
     *abort_flag = 0;
+    for (int i = 0; i < 16; ++i) reinterpret_cast<Cleared*>(smem + Map::kBad)[i].seg = -1;
     tc::mbar_fence_init();
   }
   if (warp == 1) {
@@ -514,14 +538,14 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
           if constexpr (BITS == 16) {
             const int s = it % NS;
             const uint32_t par = (it / NS - 1) & 1;
-            if (it >= NS && !tc::mbar_wait(k_empty(s), par)) { ok = false; break; }
+            if (it >= NS && !bar_wait(k_empty(s), par)) { ok = false; break; }
             const uint32_t kb = sb + Map::kK + s * Map::kKBytes;
             tc::mbar_expect_tx(k_full(s), Map::kKBytes);
 #pragma unroll
             for (int h = 0; h < Map::kHalves; ++h)
               tc::tma_load_4d(kb + h * kTK * 128, &ta.tm[0], h * 128, p0, sg.g, sg.b, k_full(s));
             k_iss = it + 1;
-            if (it >= NS && !tc::mbar_wait(v_empty(s), par)) { ok = false; break; }
+            if (it >= NS && !bar_wait(v_empty(s), par)) { ok = false; break; }
             const uint32_t vb = sb + Map::kV + s * Map::kVBytes;
             tc::mbar_expect_tx(v_full(s), Map::kVBytes);
 #pragma unroll
@@ -531,7 +555,7 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
             v_iss = it + 1;
           } else {
             const int s = it % ta.raw_stages;
-            if (it >= ta.raw_stages && !tc::mbar_wait(raw_empty(s), (it / ta.raw_stages - 1) & 1)) { ok = false; break; }
+            if (it >= ta.raw_stages && !bar_wait(raw_empty(s), (it / ta.raw_stages - 1) & 1)) { ok = false; break; }
             const int rows = min(kTK, a.cap - p0);
             const int64_t row = ((int64_t)sg.b * a.HKV + sg.g) * a.cap + p0;
             const uint32_t cb = rows * ta.code_bytes, gb = rows * ta.group_bytes;
@@ -554,9 +578,9 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
       // the copies issued last on each stage have landed before the CTA may exit
       const int ring = BITS == 16 ? NS : ta.raw_stages;
       for (int j = max(0, k_iss - ring); j < k_iss; ++j)
-        if (!tc::mbar_wait(BITS == 16 ? k_full(j % ring) : raw_full(j % ring), (j / ring) & 1)) *abort_flag = 1;
+        if (!bar_wait(BITS == 16 ? k_full(j % ring) : raw_full(j % ring), (j / ring) & 1)) *abort_flag = 1;
       for (int j = max(0, v_iss - ring); j < v_iss; ++j)
-        if (!tc::mbar_wait(v_full(j % ring), (j / ring) & 1)) *abort_flag = 1;
+        if (!bar_wait(v_full(j % ring), (j / ring) & 1)) *abort_flag = 1;
     }
   } else if (warp == 1) {
     if (lane == 0) {  // ---- MMAs ----
@@ -564,7 +588,7 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
       constexpr uint32_t idesc_pv = tc::idesc_f16_f32(kTR, 2 * D, true, false, kBf16);
       auto issue_qk = [&](int it) -> bool {
         const int s = it % NS;
-        if (!tc::mbar_wait(k_full(s), (it / NS) & 1)) return false;
+        if (!bar_wait(k_full(s), (it / NS) & 1)) return false;
         tc::tc_fence_after();
         const uint32_t kb = sb + Map::kK + s * Map::kKBytes;
 #pragma unroll
@@ -579,11 +603,11 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
       int it = 0, seg = 0;
       bool ok = true;
       for (; ok && next_segment(a, sched, sg); ++seg) {
-        ok = tc::mbar_wait(q_full, seg & 1) && issue_qk(it);
+        ok = bar_wait(q_full, seg & 1) && issue_qk(it);
         for (int kt = sg.t0; ok && kt < sg.t1; ++kt, ++it) {
           if (*abort_flag || (kt + 1 < sg.t1 && !issue_qk(it + 1))) { ok = false; break; }
           const int s = it % NS;
-          if (!tc::mbar_wait(p_full(it & 1), (it >> 1) & 1) || !tc::mbar_wait(v_full(s), (it / NS) & 1)) {
+          if (!bar_wait(p_full(it & 1), (it >> 1) & 1) || !bar_wait(v_full(s), (it / NS) & 1)) {
             ok = false;
             break;
           }
@@ -593,27 +617,31 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
           for (int kk = 0; kk < kTK / 16; ++kk)
             tc::mma_f16(tmem + kColO, tc::desc_kmajor_sw128(pb + kk * 32),
                         tc::desc_mnmajor_sw128(vb + kk * 2048, kTK * 128, 1024), idesc_pv, kt > sg.t0 || kk > 0);
-          tc::mma_commit(o_bar);
+          tc::mma_commit(o_done(it & 1));
           tc::mma_commit(v_empty(s));
         }
       }
       if (!ok) *abort_flag = 1;
       // every MMA this thread issued completes before tensor memory can be freed
       tc::mma_commit(drain);
-      if (!tc::mbar_wait(drain, 0)) *abort_flag = 1;
+      if (!bar_wait(drain, 0)) *abort_flag = 1;
     }
     __syncwarp();
-  } else if (warp < 6) {  // ---- softmax: one thread per query row ----
-    const int q = warp & 3;  // a warp reads tensor-memory lanes 32·(warp mod 4) ..
+  } else if (warp < 10) {  // ---- softmax: one thread per query row, two groups ----
+    const int grp = warp >= 6, q = warp & 3;  // a warp reads tensor-memory lanes 32·(warp mod 4) ..
     const int r = q * 32 + lane;
     const uint32_t trow = tmem + ((uint32_t)(q * 32) << 16);
     const float mult = fabsf(a.scale_log2);
-    auto load_q = [&](const Segment& g) {
+    float* m_row = reinterpret_cast<float*>(smem + Map::kState) + r;
+    float* l_row = m_row + kTR;  // group g's sum at l_row[g * kTR]
+    Cleared* bad_all = reinterpret_cast<Cleared*>(smem + Map::kBad);
+    auto load_q = [&](const Segment& g) {  // group A the first half of the channels, B the second
       const int pr = g.rt * kTR + r;
       const T* src = static_cast<const T*>(a.q) + (((int64_t)g.b * a.HKV + g.g) * a.R + pr) * D;
       const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;  // scale < 0: −q with |scale|
 #pragma unroll
-      for (int c8 = 0; c8 < D / 8; ++c8) {
+      for (int i = 0; i < D / 16; ++i) {
+        const int c8 = grp * (D / 16) + i;
         uint4 v = make_uint4(0, 0, 0, 0);
         if (pr < a.R) {
           v = *reinterpret_cast<const uint4*>(src + c8 * 8);
@@ -628,8 +656,14 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(q_full);
     };
+    // Bounded wait of the whole warp; false once anything has run out.
+    auto wait = [&](uint32_t b, int phase) {
+      const bool got = bar_wait(b, phase & 1);
+      return !__any_sync(0xffffffffu, !got || *abort_flag);
+    };
     bool alive = true;
     int it = 0, seg = 0;
+    int handed = 0, joined = 0;  // phases of m_next and l_both: a warp without a row takes no part in a segment's
     Segment nx;
     bool more = next_segment(a, sched, nx);
     if (more) load_q(nx);
@@ -640,65 +674,65 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
       const bool work = sg.rt * kTR + q * 32 < a.R;  // this warp has a row
       const int t = live ? pr % a.T : 0;
       const int ctx = sg.n - a.T;
-      uint32_t(*bad)[8] = reinterpret_cast<uint32_t(*)[8]>(smem + Map::kBad + (seg & 1) * 4 * 8 * 4);
-      if (lane < 8) bad[q][lane] = 0;
-      __syncwarp();
-      float m_ref = -INFINITY, l = 0.f;
-      for (int kt = sg.t0; alive && kt < sg.t1; ++kt, ++it) {
-        const int s = it & 1, p0 = kt * kTK;
+      float m_mine = -INFINITY, l = 0.f;  // the maximum that l refers to
+      for (int kt = sg.t0; kt < sg.t1; ++kt, ++it) {
+        if ((it & 1) != grp || !alive) continue;
+        const int p0 = kt * kTK;
         const bool tail = p0 + kTK > ctx;  // drafted rows or the cache's end in this tile
         uint64_t vis = 0;
         if (tail && live) vis = visible<kTK>(a, sg.b, t, sg.n, p0);
-        const bool got = tc::mbar_wait(s_full(s), (it >> 1) & 1);
-        if (__any_sync(0xffffffffu, !got || *abort_flag)) {
-          alive = false;
-          break;
-        }
+        if (!(alive = wait(s_full(grp), it >> 1))) continue;
         tc::tc_fence_after();
-        uint32_t pk[32];
+        const uint32_t ts = trow + kColS + 64 * grp;
+        uint8_t* prow = smem + Map::kP + grp * kTR * 128 + r * 128;
         bool need = false;
-        float factor = 1.f;
-        if (work) {
-          uint32_t sv[2][32];
-          tc::tmem_ld32(trow + kColS + 64 * s, sv[0]);
-          tc::tmem_ld32(trow + kColS + 64 * s + 32, sv[1]);
+        float factor = 1.f, mb = 0.f, mul = mult;
+        constexpr bool kKeep = BITS == 16;  // registers for all 64 columns; else they are read twice
+        float sv[kKeep ? 2 : 1][32];
+        auto load_s = [&](int h, float (&x)[32]) {
+          uint32_t u[32];
+          tc::tmem_ld32(ts + 32 * h, u);
           tc::tmem_ld_wait();
-          float mul = mult, m_tile = -INFINITY;
           if (tail) {
-            mul = 1.f;
+            const uint32_t v = (uint32_t)(vis >> (32 * h));
 #pragma unroll
-            for (int c = 0; c < 64; ++c) {
-              const float x = __uint_as_float(sv[c >> 5][c & 31]) * mult;
-              sv[c >> 5][c & 31] = __float_as_uint((vis >> c) & 1 ? x : -INFINITY);
-            }
+            for (int c = 0; c < 32; ++c) x[c] = (v >> c) & 1 ? __uint_as_float(u[c]) * mult : -INFINITY;
+          } else {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) x[c] = __uint_as_float(u[c]);
           }
+        };
+        if (work) {
+          if (tail) mul = 1.f;
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int c = 0; c < 64; ++c) m_tile = fmaxf(m_tile, __uint_as_float(sv[c >> 5][c & 31]));
+          for (int h = 0; h < 2; ++h) {
+            load_s(h, sv[kKeep ? h : 0]);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], sv[kKeep ? h : 0][c]);
+          }
+          float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           m_tile = m_tile == -INFINITY ? -INFINITY : m_tile * mul;
-          need = m_tile > m_ref + 8.f;
-          if (need) {
-            factor = ex2(m_ref - m_tile);  // 0 at the first visible key
-            m_ref = m_tile;
+          float m_prev = -INFINITY;
+          if (kt > sg.t0) {
+            if (!(alive = wait(m_next(grp ^ 1, q), handed++))) continue;
+            m_prev = *m_row;
           }
-          l *= factor;
-          const float mb = m_ref == -INFINITY ? 0.f : m_ref;
-          float ps[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < 64; c += 2) {
-            const float e0 = ex2(fmaf(__uint_as_float(sv[c >> 5][c & 31]), mul, -mb));
-            const float e1 = ex2(fmaf(__uint_as_float(sv[c >> 5][(c & 31) + 1]), mul, -mb));
-            ps[(c >> 1) & 3] += e0 + e1;
-            pk[c >> 1] = pack2<T>(e0, e1);  // P in the type: one rounding of each weight
+          need = m_tile > m_prev + 8.f;
+          const float m_new = need ? m_tile : m_prev;
+          *m_row = m_new;
+          if (kt + 1 < sg.t1) {
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(m_next(grp, q));
           }
-          l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+          if (need) factor = ex2(m_prev - m_new);  // 0 at the first visible key
+          if (m_new != m_mine) l *= ex2(m_mine - m_new);
+          m_mine = m_new;
+          mb = m_new == -INFINITY ? 0.f : m_new;
         }
         if (tail) {  // clear the V rows a zero weight may not meet
           const int st = it % NS;
-          const bool vok = tc::mbar_wait(v_full(st), (it / NS) & 1);
-          if (__any_sync(0xffffffffu, !vok)) {
-            alive = false;
-            break;
-          }
+          if (!(alive = wait(v_full(st), it / NS))) continue;
           const int vr = q * 16 + (lane >> 1), pos = p0 + vr;
           bool clear = pos >= sg.n;
           uint8_t* vrow = smem + Map::kV + st * Map::kVBytes + (lane & 1) * Map::kHalves * kTK * 128 + vr * 128;
@@ -706,7 +740,7 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
             bool nf = false;
 #pragma unroll
             for (int h = 0; h < Map::kHalves; ++h)
-#pragma unroll
+#pragma unroll 4
               for (int c = 0; c < 8; ++c) {
                 const uint4 v = *reinterpret_cast<const uint4*>(vrow + h * kTK * 128 + c * 16);
                 nf |= nonfinite2<T>(v.x) | nonfinite2<T>(v.y) | nonfinite2<T>(v.z) | nonfinite2<T>(v.w);
@@ -717,168 +751,195 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
           if (clear) {
 #pragma unroll
             for (int h = 0; h < Map::kHalves; ++h)
-#pragma unroll
+#pragma unroll 4
               for (int c = 0; c < 8; ++c)
                 *reinterpret_cast<uint4*>(vrow + h * kTK * 128 + c * 16) = make_uint4(0, 0, 0, 0);
-            if (pos < sg.n && (lane & 1) == 0) atomicOr(&bad[q][(pos - ctx) >> 5], 1u << ((pos - ctx) & 31));
+          }
+          const bool drafted = clear && pos < sg.n;
+          if (__any_sync(0xffffffffu, drafted)) {
+            // The slot was last read two segments ago; this segment's first S, which needs every warp's Q of
+            // it, came after that.
+            Cleared* mine = bad_all + (seg & 1) * 8 + grp * 4 + q;
+            if (mine->seg != seg && lane < 8) mine->bits[lane] = 0;
+            __syncwarp();
+            if (lane == 0) mine->seg = seg;
+            if (drafted && (lane & 1) == 0) atomicOr(&mine->bits[(pos - ctx) >> 5], 1u << ((pos - ctx) & 31));
           }
         }
-        // O and the P buffer are free once the last P·V has completed
-        if (kt > sg.t0) {
-          const bool done = tc::mbar_wait(o_bar, (it - 1) & 1);
-          if (__any_sync(0xffffffffu, !done)) {
-            alive = false;
-            break;
-          }
-          tc::tc_fence_after();
-          if (__any_sync(0xffffffffu, need)) {
-#pragma unroll 1
-            for (int cb = 0; cb < 2 * D / 32; ++cb) {
-              uint32_t ov[32];
-              tc::tmem_ld32(trow + kColO + cb * 32, ov);
-              tc::tmem_ld_wait();
-#pragma unroll
-              for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * factor);
-              tc::tmem_st32(trow + kColO + cb * 32, ov);
-            }
-            tc::tmem_st_wait();
-          }
-        }
+        // the P buffer is free once this group's last P·V has completed
+        if (it >= 2 && !(alive = wait(o_done(grp), (it - 2) >> 1))) continue;
         if (work) {
-          uint8_t* prow = smem + Map::kP + s * kTR * 128 + r * 128;
+          float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int c8 = 0; c8 < 8; ++c8)
-            *reinterpret_cast<uint4*>(prow + ((c8 ^ (r & 7)) << 4)) =
-                make_uint4(pk[4 * c8], pk[4 * c8 + 1], pk[4 * c8 + 2], pk[4 * c8 + 3]);
+          for (int h = 0; h < 2; ++h) {
+            float(&x)[32] = sv[kKeep ? h : 0];
+            if constexpr (!kKeep) load_s(h, x);
+#pragma unroll
+            for (int c8 = 0; c8 < 4; ++c8) {
+              uint32_t pk[4];
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                const float e0 = ex2(fmaf(x[8 * c8 + 2 * c], mul, -mb)), e1 = ex2(fmaf(x[8 * c8 + 2 * c + 1], mul, -mb));
+                ps[c] += e0 + e1;
+                pk[c] = pack2<T>(e0, e1);  // P in the type: one rounding of each weight
+              }
+              *reinterpret_cast<uint4*>(prow + (((4 * h + c8) ^ (r & 7)) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+            }
+          }
+          l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+        }
+        // O takes a raised maximum once the last tile's P·V has completed
+        if (kt > sg.t0 && __any_sync(0xffffffffu, need)) {
+          if (!(alive = wait(o_done(grp ^ 1), (it - 1) >> 1))) continue;
+          tc::tc_fence_after();
+#pragma unroll 1
+          for (int cb = 0; cb < 2 * D / 32; ++cb) {
+            uint32_t ov[32];
+            tc::tmem_ld32(trow + kColO + cb * 32, ov);
+            tc::tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * factor);
+            tc::tmem_st32(trow + kColO + cb * 32, ov);
+          }
+          tc::tmem_st_wait();
         }
         tc::fence_proxy_async_smem();
         tc::tc_fence_before();
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(p_full(s));
+        if (lane == 0) tc::mbar_arrive(p_full(grp));
       }
       more = next_segment(a, sched, nx);
-      // the segment's last S is complete: its Q is free, and the next one's first product can start
+      const int e = it - 1;  // the segment's last tile
+      if (alive) alive = wait(s_full(e & 1), e >> 1);
+      // its S is complete: Q is free, and the next segment's first product can start
       if (more && alive) load_q(nx);
-      if (alive) alive = __all_sync(0xffffffffu, tc::mbar_wait(o_bar, (it - 1) & 1));
-      if (!alive) *abort_flag = 1;
+      if (alive) alive = wait(o_done(e & 1), e >> 1);
       tc::tc_fence_after();
       if (work) {
-        // Through this warp's 4 KB of the P buffer of the next tile's other half: the last P·V has read it.
+        float m_ref = -INFINITY;
+        if (alive) {  // both groups' sums at the last maximum
+          m_ref = *m_row;
+          if (m_ref != m_mine) l *= ex2(m_mine - m_ref);
+          l_row[grp * kTR] = l;
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(l_both(q));
+          alive = wait(l_both(q), joined++);
+          l = l_row[0] + l_row[kTR];
+        }
+        // Through this warp's 4 KB of its group's P buffer: its last P·V is complete.
         const float inv = !alive ? NAN : l == 0.f ? 0.f : 1.f / l;
-        uint8_t* stage = smem + Map::kP + q * 32 * 128;
+        uint8_t* stage = smem + Map::kP + grp * kTR * 128 + q * 32 * 128;
         const int64_t row0 = ((int64_t)sg.b * a.HKV + sg.g) * a.R + sg.rt * kTR + q * 32;  // first of the warp's rows
         const int rows = min(32, a.R - (sg.rt * kTR + q * 32));
-        uint32_t any_bad = 0;
+        const Cleared* bad = bad_all + (seg & 1) * 8;
+        bool any_bad = false;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) any_bad |= bad[0][w] | bad[1][w] | bad[2][w] | bad[3][w];
-        if (sg.slot >= 0 && live) {
+        for (int w = 0; w < 8; ++w) any_bad |= bad[w].seg == seg;
+        if (sg.slot >= 0 && live && grp == 0) {
           float* ml = a.part_ml + ((int64_t)sg.slot * a.slot_rows + r) * 2;
           ml[0] = m_ref;
           ml[1] = alive ? l : NAN;
         }
-        if (any_bad && alive) {  // any_bad is the same in the whole CTA
-          T* yrow = live && sg.slot < 0 ? static_cast<T*>(a.y) + (row0 + lane) * 2 * D : nullptr;
-          float* orow = live && sg.slot >= 0 ? a.part_o + ((int64_t)sg.slot * a.slot_rows + r) * 2 * D : nullptr;
-          finish_cleared<T, D, BITS>(a, sg.b, sg.g, bad, live ? pr : 0, ctx, m_ref, inv, trow + kColO, yrow, orow);
-        } else
+        const int cb0 = grp * (D / 32);
+        {
 #pragma unroll 1
-        for (int cb = 0; cb < 2 * D / 32; ++cb) {
-          uint32_t ov[32];
-          tc::tmem_ld32(trow + kColO + cb * 32, ov);
-          tc::tmem_ld_wait();
-          float o[32];
+          for (int cb = cb0; cb < cb0 + D / 32; ++cb) {
+            uint32_t ov[32];
+            tc::tmem_ld32(trow + kColO + cb * 32, ov);
+            tc::tmem_ld_wait();
+            float o[32];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[(e & ~7) + chunk_channel<BITS>(e & 7)] = alive ? __uint_as_float(ov[e]) : NAN;
-          if (sg.slot < 0) {  // 32 rows × 64 bytes
+            for (int i = 0; i < 32; ++i) o[(i & ~7) + chunk_channel<BITS>(i & 7)] = alive ? __uint_as_float(ov[i]) : NAN;
+            if (sg.slot < 0) {  // 32 rows × 64 bytes
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              uint4 v;
-              v.x = pack2<T>(o[8 * c] * inv, o[8 * c + 1] * inv);
-              v.y = pack2<T>(o[8 * c + 2] * inv, o[8 * c + 3] * inv);
-              v.z = pack2<T>(o[8 * c + 4] * inv, o[8 * c + 5] * inv);
-              v.w = pack2<T>(o[8 * c + 6] * inv, o[8 * c + 7] * inv);
-              *reinterpret_cast<uint4*>(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = v;
+              for (int c = 0; c < 4; ++c) {
+                uint4 v;
+                v.x = pack2<T>(o[8 * c] * inv, o[8 * c + 1] * inv);
+                v.y = pack2<T>(o[8 * c + 2] * inv, o[8 * c + 3] * inv);
+                v.z = pack2<T>(o[8 * c + 4] * inv, o[8 * c + 5] * inv);
+                v.w = pack2<T>(o[8 * c + 6] * inv, o[8 * c + 7] * inv);
+                *reinterpret_cast<uint4*>(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = v;
+              }
+              __syncwarp();
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int rr = i * 8 + (lane >> 2), c = lane & 3;
+                const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 64 + ((c ^ ((rr >> 1) & 3)) << 4));
+                if (rr < rows)
+                  *reinterpret_cast<uint4*>(static_cast<T*>(a.y) + (row0 + rr) * 2 * D + cb * 32 + c * 8) = v;
+              }
+            } else {  // 32 rows × 128 bytes
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                *reinterpret_cast<float4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+                    make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+              __syncwarp();
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int rr = i * 4 + (lane >> 3), c = lane & 7;
+                const float4 v = *reinterpret_cast<const float4*>(stage + rr * 128 + ((c ^ (rr & 7)) << 4));
+                if (rr < rows)
+                  *reinterpret_cast<float4*>(a.part_o + ((int64_t)sg.slot * a.slot_rows + q * 32 + rr) * 2 * D + cb * 32 +
+                                             c * 4) = v;
+              }
             }
             __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int rr = i * 8 + (lane >> 2), c = lane & 3;
-              const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 64 + ((c ^ ((rr >> 1) & 3)) << 4));
-              if (rr < rows)
-                *reinterpret_cast<uint4*>(static_cast<T*>(a.y) + (row0 + rr) * 2 * D + cb * 32 + c * 8) = v;
-            }
-          } else {  // 32 rows × 128 bytes
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-              *reinterpret_cast<float4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) =
-                  make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int rr = i * 4 + (lane >> 3), c = lane & 7;
-              const float4 v = *reinterpret_cast<const float4*>(stage + rr * 128 + ((c ^ (rr & 7)) << 4));
-              if (rr < rows)
-                *reinterpret_cast<float4*>(a.part_o + ((int64_t)sg.slot * a.slot_rows + q * 32 + rr) * 2 * D + cb * 32 +
-                                           c * 4) = v;
-            }
           }
-          __syncwarp();
         }
+        if (any_bad && alive && live)
+          add_cleared<T, D, BITS>(a, sg.b, sg.g, bad, seg, pr, t, ctx, m_ref, inv, grp,
+                                  sg.slot < 0 ? static_cast<T*>(a.y) + (row0 + lane) * 2 * D : nullptr,
+                                  a.part_o + ((int64_t)max(sg.slot, 0) * a.slot_rows + r) * 2 * D);
       }
+      if (!alive) *abort_flag = 1;
       ++seg;
     }
   } else if constexpr (BITS != 16) {  // ---- operand tiles from packed rows ----
-    const int tid = threadIdx.x - 192;
+    const int tid = threadIdx.x - 320;
+    const int gs_log = 31 - __clz(a.gs);  // the group size divides 64 or 128
     constexpr int kUnits = kTK * D / 32;  // 32 channels of one row
-    auto fill = [&](const uint8_t* codes, const uint8_t* scales, uint8_t* tile) {
-      for (int u = tid; u < kUnits; u += 256) {
-        const int row = u / (D / 32), c32 = u % (D / 32);
-        // the four chunks' order differs between a row's halves so that eight lanes write to eight bank groups
-        const int flip = D == 128 ? (c32 >> 1) << 1 : 0;
-        uint32_t w[BITS];
-        const uint4* src = reinterpret_cast<const uint4*>(codes + row * ta.code_bytes + c32 * BITS * 4);
-#pragma unroll
-        for (int i = 0; i < BITS / 4; ++i) *reinterpret_cast<uint4*>(w + 4 * i) = src[i];
-        const T* sc = reinterpret_cast<const T*>(scales + row * ta.group_bytes);
-        const T* bi = reinterpret_cast<const T*>(scales + kTK * ta.group_bytes + row * ta.group_bytes);
-        T s = sc[c32 * 32 / a.gs], b = bi[c32 * 32 / a.gs];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int kx = k ^ flip;
-          uint32_t w0, w1 = 0;
-          if constexpr (BITS == 4) {
-            w0 = flip ? w[k ^ 2] : w[k];
-          } else {
-            w0 = flip ? w[2 * (k ^ 2)] : w[2 * k];
-            w1 = flip ? w[2 * (k ^ 2) + 1] : w[2 * k + 1];
-          }
-          const int c8 = c32 * 4 + kx;
-          if (a.gs < 32) s = sc[c8 * 8 / a.gs], b = bi[c8 * 8 / a.gs];
-          *reinterpret_cast<uint4*>(tile + (c8 >> 3) * kTK * 128 + row * 128 + (((c8 & 7) ^ (row & 7)) << 4)) =
-              dequant8<T, BITS>(w0, w1, s, b);
-        }
-      }
-      tc::fence_proxy_async_smem();
-      __syncwarp();
-    };
     int it = 0;
     bool alive = true;
     while (alive && next_segment(a, sched, sg)) {
       for (int kt = sg.t0; kt < sg.t1; ++kt, ++it) {
         const int rs = it % ta.raw_stages, s = it % NS;
         const uint32_t par = (it / NS - 1) & 1;
-        bool ok = tc::mbar_wait(raw_full(rs), (it / ta.raw_stages) & 1) && (it < NS || tc::mbar_wait(k_empty(s), par));
+        const bool ok = bar_wait(raw_full(rs), (it / ta.raw_stages) & 1) &&
+                        (it < NS || (bar_wait(k_empty(s), par) && bar_wait(v_empty(s), par)));
         if (__any_sync(0xffffffffu, !ok || *abort_flag)) { alive = false; break; }
         const uint8_t* raw = smem + Map::kRaw + rs * (3 * kTK * ta.code_bytes + 6 * kTK * ta.group_bytes);
-        const uint8_t* rsc = raw + 3 * kTK * ta.code_bytes;
-        fill(raw, rsc, smem + Map::kK + s * Map::kKBytes);
-        if (lane == 0) tc::mbar_arrive(k_full(s));
-        ok = it < NS || tc::mbar_wait(v_empty(s), par);
-        if (__any_sync(0xffffffffu, !ok)) { alive = false; break; }
-        uint8_t* vt = smem + Map::kV + s * Map::kVBytes;
-        fill(raw + kTK * ta.code_bytes, rsc + 2 * kTK * ta.group_bytes, vt);
-        fill(raw + 2 * kTK * ta.code_bytes, rsc + 4 * kTK * ta.group_bytes, vt + Map::kKBytes);
+        for (int u = tid; u < 3 * kUnits; u += Cfg::kThreads - 320) {  // 3·kUnits is a multiple of the threads
+          const int slot = u / kUnits, row = u % kUnits / (D / 32), c32 = u % (D / 32);
+          const uint8_t* codes = raw + (slot * kTK + row) * ta.code_bytes + c32 * BITS * 4;
+          const uint8_t* scales = raw + 3 * kTK * ta.code_bytes + (slot * 2 * kTK + row) * ta.group_bytes;
+          uint8_t* tile = smem + (slot == 0 ? Map::kK + s * Map::kKBytes : Map::kV + s * Map::kVBytes + (slot - 1) * Map::kKBytes);
+          // the four chunks' order differs between a row's halves so that eight lanes write to eight bank groups
+          const int flip = D == 128 ? (c32 >> 1) << 1 : 0;
+          uint32_t w[BITS];
+#pragma unroll
+          for (int i = 0; i < BITS / 4; ++i) *reinterpret_cast<uint4*>(w + 4 * i) = reinterpret_cast<const uint4*>(codes)[i];
+          const T* sc = reinterpret_cast<const T*>(scales);
+          const T* bi = reinterpret_cast<const T*>(scales + kTK * ta.group_bytes);
+          T sv = sc[c32 * 32 >> gs_log], bv = bi[c32 * 32 >> gs_log];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t w0, w1 = 0;
+            if constexpr (BITS == 4) {
+              w0 = flip ? w[k ^ 2] : w[k];
+            } else {
+              w0 = flip ? w[2 * (k ^ 2)] : w[2 * k];
+              w1 = flip ? w[2 * (k ^ 2) + 1] : w[2 * k + 1];
+            }
+            const int c8 = c32 * 4 + (k ^ flip);
+            if (gs_log < 5) sv = sc[c8 * 8 >> gs_log], bv = bi[c8 * 8 >> gs_log];
+            *reinterpret_cast<uint4*>(tile + (c8 >> 3) * kTK * 128 + row * 128 + (((c8 & 7) ^ (row & 7)) << 4)) =
+                dequant8<T, BITS>(w0, w1, sv, bv);
+          }
+        }
+        tc::fence_proxy_async_smem();
+        __syncwarp();
         if (lane == 0) {
+          tc::mbar_arrive(k_full(s));
           tc::mbar_arrive(v_full(s));
           tc::mbar_arrive(raw_empty(rs));
         }
@@ -928,28 +989,57 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__
   auto lo = [&](int64_t i) { return i * total / grid; };
   const int64_t i0 = ((s + 1) * grid - 1) / total, i1 = (e * grid - 1) / total;  // CTAs of tiles s and e − 1
   if (i0 == i1) return;  // written by its CTA
-  auto slot_row = [&](int64_t i) { return (2 * i + (lo(i) >= s ? 0 : 1)) * a.slot_rows + r; };
-  float M = -INFINITY;
-  for (int64_t i = i0; i <= i1; ++i)
-    if (lo(i) < lo(i + 1)) M = fmaxf(M, a.part_ml[slot_row(i) * 2]);
+  const int parts = (int)(i1 - i0) + 1;
+  // a lane holds one CTA's part at a time: its place, maximum and sum (an empty CTA has none)
+  auto part = [&](int k, int64_t& sr, float& m, float& l) {
+    m = -INFINITY, l = 0.f, sr = 0;
+    const int64_t i = i0 + k, at = lo(i);
+    if (k >= parts || at >= lo(i + 1)) return;
+    sr = (2 * i + (at >= s ? 0 : 1)) * a.slot_rows + r;
+    const float2 f = *reinterpret_cast<const float2*>(a.part_ml + sr * 2);
+    m = f.x, l = f.y;
+  };
+  int64_t sr;
+  float m, l, M = -INFINITY;
+  for (int k0 = 0; k0 < parts; k0 += 32) {
+    part(k0 + lane, sr, m, l);
+    M = fmaxf(M, m);
+  }
+  M = warp_max(M);
   float L = 0.f, o[V] = {};
-  for (int64_t i = i0; i <= i1; ++i) {
-    if (lo(i) >= lo(i + 1)) continue;
-    const int64_t sr = slot_row(i);
-    const float ms = a.part_ml[sr * 2];
-    if (ms == -INFINITY) continue;
-    const float w = exp2f(ms - M);
-    L = fmaf(w, a.part_ml[sr * 2 + 1], L);
-    const float4* p = reinterpret_cast<const float4*>(a.part_o + sr * 2 * D);
+  for (int k0 = 0; k0 < parts; k0 += 32) {
+    if (parts > 32 || k0 > 0) part(k0 + lane, sr, m, l);
+    const float w = m == -INFINITY ? 0.f : exp2f(m - M);
+    L += w == 0.f ? 0.f : w * l;
+    const int nk = min(32, parts - k0);
+    constexpr int kU = 4;  // parts in flight
+    for (int k = 0; k < nk; k += kU) {
+      float4 f[kU][V / 4];
+      float wk[kU];
 #pragma unroll
-    for (int v = 0; v < V / 4; ++v) {
-      const float4 f = p[v * 32 + lane];
-      o[4 * v] = fmaf(w, f.x, o[4 * v]);
-      o[4 * v + 1] = fmaf(w, f.y, o[4 * v + 1]);
-      o[4 * v + 2] = fmaf(w, f.z, o[4 * v + 2]);
-      o[4 * v + 3] = fmaf(w, f.w, o[4 * v + 3]);
+      for (int x = 0; x < kU; ++x) {
+        const int kk = min(k + x, nk - 1);
+        wk[x] = __shfl_sync(0xffffffffu, w, kk);
+        const int64_t srk = __shfl_sync(0xffffffffu, sr, kk);
+        if (k + x >= nk) wk[x] = 0.f;
+        if (wk[x] == 0.f) continue;
+#pragma unroll
+        for (int v = 0; v < V / 4; ++v) f[x][v] = reinterpret_cast<const float4*>(a.part_o + srk * 2 * D)[v * 32 + lane];
+      }
+#pragma unroll
+      for (int x = 0; x < kU; ++x) {
+        if (wk[x] == 0.f) continue;  // a part that saw no key of this row
+#pragma unroll
+        for (int v = 0; v < V / 4; ++v) {
+          o[4 * v] = fmaf(wk[x], f[x][v].x, o[4 * v]);
+          o[4 * v + 1] = fmaf(wk[x], f[x][v].y, o[4 * v + 1]);
+          o[4 * v + 2] = fmaf(wk[x], f[x][v].z, o[4 * v + 2]);
+          o[4 * v + 3] = fmaf(wk[x], f[x][v].w, o[4 * v + 3]);
+        }
+      }
     }
   }
+  L = warp_sum(L);
   const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
   for (int v = 0; v < V / 4; ++v) {

@@ -157,6 +157,8 @@ CASES = [
     (1, 8, 1, 64, 128, 1024, 1000, "tree"),  # 512 packed rows
     (1, 2, 1, 256, 64, 300, 300, "any"),  # the largest tree, over more than two tiles
     (3, 24, 8, 6, 128, 2304, 2200, "trees"),
+    (4, 24, 8, 43, 128, 1024, 1000, "trees"),  # several units per SM, each second one with a single row
+    (5, 6, 2, 22, 64, 4096, 4001, "tree"),
 ]
 
 
