@@ -242,8 +242,8 @@ MOTIF_API int motif_vanilla_decode_step(const void* qkv, const float* inv_freq, 
  * kv_len_dev: one length (kv_len_stride 0) or one per sequence (1), clamped to
  * [0, kv_cap]; with fewer than T live rows the tree's first rows are missing.
  * workspace: motif_sdpa_dual_v_tree_workspace_bytes of the same arguments
- * (kv_len_bound: kv_len, or kv_cap with kv_len_dev), any contents; calls that
- * may overlap need one each. err (optional device int): set to 1 if a
+ * (kv_len_bound: kv_len, or kv_cap with kv_len_dev; one_length: 0 with
+ * kv_len_stride 1, else 1), any contents; calls that may overlap need one each. err (optional device int): set to 1 if a
  * pipeline wait timed out (the rows it concerns are then NaN). */
 typedef struct motif_tree_kv {
   const void* data[3];
@@ -253,7 +253,7 @@ typedef struct motif_tree_kv {
 } motif_tree_kv;
 MOTIF_API size_t motif_sdpa_dual_v_tree_workspace_bytes(int dtype, int bits, int group_size, int64_t batch,
                                                        int64_t h_q, int64_t h_kv, int64_t tree_rows, int64_t kv_cap,
-                                                       int64_t head_dim, int64_t kv_len_bound);
+                                                       int64_t head_dim, int64_t kv_len_bound, int one_length);
 MOTIF_API int motif_sdpa_dual_v_tree(int dtype, int bits, int group_size, const void* q, const motif_tree_kv* kv,
                                      const uint8_t* tree_mask, int64_t mask_batch_stride, float scale, int64_t batch,
                                      int64_t h_q, int64_t h_kv, int64_t tree_rows, int64_t kv_cap, int64_t head_dim,

@@ -10,7 +10,7 @@
 // All GQA heads of a kv head share its rows, so the gqa·T query rows of a kv head are packed
 // (head-major) and cut into row tiles; a unit of work is (sequence, kv head, row tile) and its
 // key tiles. The tiles of all units form one line that is cut into gridDim.x equal parts
-// (Schedule), whatever the sequences' lengths: a CTA may end one unit and start the next. A unit
+// (Line, Schedule), whatever the sequences' lengths: a CTA may end one unit and start the next. A unit
 // that lies in one CTA is normalised and written by it; the others leave fp32 partials (running
 // maximum, Σp, unnormalised O) that tree_merge_kernel joins in a fixed order.
 #include <cuda.h>
@@ -38,12 +38,13 @@ struct TreeArgs {
   int len_step;             // 0: one for all sequences
   int len;
   void* y;                  // (B, HKV·gqa, T, 2D)
-  float* part_o;            // [2·grid][slot_rows][2D]
-  float* part_ml;           // [2·grid][slot_rows][2]
+  float* part_o;            // [parts][2D / 8][slot_rows][8]
+  float* part_ml;           // [parts][slot_rows][2]
   int slot_rows;            // rows of a partial: min(tile_rows, R)
   int* err;
   int B, HKV, gqa, T, R, row_tiles, cap, gs;
   int tile_rows, tile_keys;
+  int cuts;                 // > 0: every unit is cut into so many parts, grid (cuts, HKV·row_tiles, B)
   float scale_log2;
 };
 
@@ -55,75 +56,145 @@ __device__ __forceinline__ int key_tiles(const TreeArgs& a, int n) {
   return max(1, (n + a.tile_keys - 1) / a.tile_keys);  // an empty cache is one tile without a visible key
 }
 
-// Line of all units' key tiles, and this CTA's part [x, x1) of it. Every thread of a warp calls it.
+// Sequences of one length: every unit is cut into `cuts` parts, one CTA each. Otherwise the units' key tiles
+// form one line that is cut into `grid` parts of equal length; where a CTA has many tiles every unit counts
+// `lead` more than it has, since a CTA that ends one unit and begins the next pays for two loads of
+// queries and two outputs.
+constexpr int kLead = 4, kLeadTiles = 8;
+
+struct Line {
+  int total, per, rem, grid, lead;
+  __device__ __forceinline__ void init(int tiles, int units, int parts) {  // tiles of all units < 2^28: checked by the host
+    grid = parts;
+    lead = tiles >= kLeadTiles * grid ? kLead : 0;
+    total = tiles + units * lead;
+    per = total / grid;
+    rem = total - per * grid;
+  }
+  __device__ __forceinline__ int lo(int i) const { return i * per + i * rem / grid; }  // ⌊i·total / grid⌋
+  __device__ __forceinline__ int owner(int x) const {                                  // the part that holds place x
+    int i = (int)((float)x * (float)grid / (float)total);
+    i = min(max(i, 0), grid - 1);
+    while (i > 0 && lo(i) > x) --i;
+    while (i + 1 < grid && lo(i + 1) <= x) ++i;
+    return i;
+  }
+};
+
+__device__ __forceinline__ int cut_at(int k, int nt, int cuts) { return (int)((unsigned)k * (unsigned)nt / (unsigned)cuts); }
+
+// This CTA's share of one unit: key tiles [t0, t1) of row tile rt of kv head g of sequence b.
+struct Segment {
+  int b, g, rt, n, t0, t1;
+  int slot;  // its partial's place; -1: the whole unit
+};
+
+// Walks this CTA's part of the line. Every thread of a warp constructs it.
 struct Schedule {
-  int x0, x, x1;
-  int b, base;  // sequence of x, its first tile
-  int n, nt;    // its live rows and key tiles per unit
+  int x0, x1;     // the part
+  int at, nt, n;  // the current unit's place, key tiles, live rows
+  int b, g, rt, lead;
 
   __device__ __forceinline__ Schedule(const TreeArgs& a) {
-    const int lane = threadIdx.x & 31;
+    if (a.cuts) {
+      n = live_rows(a, 0);
+      nt = key_tiles(a, n);
+      b = blockIdx.z;
+      g = blockIdx.y / a.row_tiles;
+      rt = blockIdx.y - g * a.row_tiles;
+      at = 0;
+      x0 = cut_at(blockIdx.x, nt, a.cuts);
+      x1 = cut_at(blockIdx.x + 1, nt, a.cuts);
+      return;
+    }
     const int per_b = a.HKV * a.row_tiles;
-    int total = 0;  // < 2^31: checked by the host for the longest lengths
-    for (int i = lane; i < a.B; i += 32) total += key_tiles(a, live_rows(a, i));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    total *= per_b;
-    x0 = x = (int)((int64_t)blockIdx.x * total / gridDim.x);
-    x1 = (int)((int64_t)(blockIdx.x + 1) * total / gridDim.x);
-    b = base = 0;
-    for (;;) {  // the sequence that holds tile x
+    int tiles = 0;
+    for (int i = threadIdx.x & 31; i < a.B; i += 32) tiles += key_tiles(a, live_rows(a, i));
+    tiles = (int)__reduce_add_sync(0xffffffffu, (unsigned)tiles) * per_b;
+    Line line;
+    line.init(tiles, a.B * per_b, gridDim.x);
+    lead = line.lead;
+    x0 = line.lo(blockIdx.x);
+    x1 = line.lo(blockIdx.x + 1);
+    b = 0, at = 0;
+    for (;;) {  // the sequence and unit of place x0
       n = live_rows(a, b);
       nt = key_tiles(a, n);
-      if (b + 1 >= a.B || x < base + nt * per_b) return;
-      base += nt * per_b;
+      const int len = (nt + lead) * per_b;
+      if (b + 1 >= a.B || x0 < at + len) break;
+      at += len;
       ++b;
+    }
+    const int u = (x0 - at) / (nt + lead);
+    at += u * (nt + lead);
+    g = u / a.row_tiles;
+    rt = u - g * a.row_tiles;
+  }
+  __device__ __forceinline__ bool next(const TreeArgs& a, Segment& s) {
+    if (a.cuts) {
+      if (at || x0 >= x1) return false;
+      at = 1;
+      s.b = b, s.g = g, s.rt = rt, s.n = n;
+      s.t0 = x0, s.t1 = x1;
+      s.slot = x0 == 0 && x1 == nt ? -1 : (int)((blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x);
+      return true;
+    }
+    for (;;) {
+      if (at >= x1 || b >= a.B) return false;
+      s.t0 = max(x0 - at - lead, 0);
+      s.t1 = min(x1 - at - lead, nt);
+      s.b = b, s.g = g, s.rt = rt, s.n = n;
+      // at most two segments of a CTA are parts of units: one begun before it, and its last
+      s.slot = s.t0 == 0 && s.t1 == nt ? -1 : 2 * (int)blockIdx.x + (s.t0 > 0 ? 0 : 1);
+      at += nt + lead;
+      if (++rt == a.row_tiles) {
+        rt = 0;
+        if (++g == a.HKV) {
+          g = 0;
+          if (++b < a.B) {
+            n = live_rows(a, b);
+            nt = key_tiles(a, n);
+          }
+        }
+      }
+      if (s.t1 > s.t0) return true;
     }
   }
 };
 
-// One CTA's share of one unit: key tiles [t0, t1) of row tile rt of kv head g of sequence b.
-struct Segment {
-  int b, g, rt, n, t0, t1;
-  int slot;    // its partial's place; -1: the unit lies in this CTA
-};
-
-__device__ __forceinline__ bool next_segment(const TreeArgs& a, Schedule& s, Segment& g) {
-  if (s.x >= s.x1) return false;
-  const int per_b = a.HKV * a.row_tiles;
-  if (s.x >= s.base + s.nt * per_b) {
-    s.base += s.nt * per_b;
-    ++s.b;
-    s.n = live_rows(a, s.b);
-    s.nt = key_tiles(a, s.n);
-  }
-  const int in = s.x - s.base, u = in / s.nt;
-  g.b = s.b;
-  g.n = s.n;
-  g.g = u / a.row_tiles;
-  g.rt = u - g.g * a.row_tiles;
-  g.t0 = in - u * s.nt;
-  g.t1 = min(s.nt, g.t0 + (s.x1 - s.x));
-  // at most two segments of a CTA are parts of units: the first (a unit begun before it) and the last
-  g.slot = g.t0 == 0 && g.t1 == s.nt ? -1 : 2 * (int)blockIdx.x + (s.x == s.x0 ? 0 : 1);
-  s.x += g.t1 - g.t0;
-  return true;
+// Place of eight channels (chunk c8) of a partial's row: a warp of rows writes whole lines.
+template <int D>
+__device__ __forceinline__ int64_t part_at(const TreeArgs& a, int slot, int c8, int row) {
+  return (((int64_t)slot * (2 * D / 8) + c8) * a.slot_rows + row) * 8;
 }
 
-// Bit c: row t of sequence b sees cache row p0 + c, c < NB.
-template <int NB>
-__device__ __forceinline__ uint64_t visible(const TreeArgs& a, int b, int t, int n, int p0) {
-  const int ctx = n - a.T;  // negative where fewer than T rows are live
+// Tree rows that row t of sequence b sees, j0 ≤ j < j0 + 64, as bits.
+__device__ __forceinline__ uint64_t mask_bits(const TreeArgs& a, int b, int t, int j0) {
+  if (!a.mask) return t < j0 ? 0 : t - j0 >= 63 ? ~0ull : (2ull << (t - j0)) - 1;
+  const uint8_t* m = a.mask + b * a.mask_b + (int64_t)t * a.T;
   uint64_t w = 0;
-  const uint8_t* m = a.mask ? a.mask + b * a.mask_b + (int64_t)t * a.T : nullptr;
-#pragma unroll 16
-  for (int c = 0; c < NB; ++c) {
-    const int pos = p0 + c, j = pos - ctx;
-    bool v = pos < n;
-    if (v && j >= 0) v = m ? m[j] != 0 : j <= t;
-    w |= (uint64_t)v << c;
+  if ((((reinterpret_cast<uintptr_t>(m) + j0) | (a.T - j0)) & 7) == 0) {  // whole 8-byte words
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint64_t x = j0 + 8 * i < a.T ? *reinterpret_cast<const uint64_t*>(m + j0 + 8 * i) : 0;
+      x |= x >> 4, x |= x >> 2, x |= x >> 1;  // bit 0 of a byte: the byte is not 0 …
+      w |= ((x & 0x0101010101010101ull) * 0x0102040810204080ull >> 56) << (8 * i);  // … eight of them side by side
+    }
+    return w;
   }
+#pragma unroll 16
+  for (int c = 0; c < 64; ++c)
+    if (j0 + c < a.T) w |= (uint64_t)(m[j0 + c] != 0) << c;
   return w;
+}
+
+// Bit c: the row sees cache row p0 + c, c < 64, of n live ones; row: its mask_bits from 0 (used where T ≤ 64).
+__device__ __forceinline__ uint64_t visible(const TreeArgs& a, uint64_t row, int b, int t, int ctx, int p0) {
+  const int j0 = p0 - ctx;  // tree row of cache row p0
+  if (j0 <= -64) return ~0ull;
+  if (a.T > 64) row = mask_bits(a, b, t, max(j0, 0));
+  else if (j0 > 0) row = j0 > 63 ? 0 : row >> j0;
+  return j0 < 0 ? row << -j0 | ((1ull << -j0) - 1) : row;  // the context, then the tree
 }
 
 // Eight consecutive channels [8·c8, 8·c8 + 8) of row `pos` of slot s (kv head g of sequence b) in fp32.
@@ -179,7 +250,7 @@ __global__ void __launch_bounds__(kSThreads, 2) tree_simt_kernel(const __grid_co
 
   Schedule sched(a);
   Segment sg;
-  while (next_segment(a, sched, sg)) {
+  while (sched.next(a, sg)) {
     const int64_t qrow = ((int64_t)sg.b * a.HKV + sg.g) * a.R + sg.rt * kSR;  // first packed row of the tile
     const int rows = min(kSR, a.R - sg.rt * kSR);
     __syncthreads();
@@ -278,7 +349,7 @@ __global__ void __launch_bounds__(kSThreads, 2) tree_simt_kernel(const __grid_co
       if (sg.slot < 0)
         static_cast<T*>(a.y)[(qrow + row0 + r) * 2 * D + ch] = from_f<T>(acc[r] * inv_l[row0 + r]);
       else
-        a.part_o[((int64_t)sg.slot * a.slot_rows + row0 + r) * 2 * D + ch] = acc[r];
+        a.part_o[part_at<D>(a, sg.slot, ch >> 3, row0 + r) + (ch & 7)] = acc[r];
     }
   }
 }
@@ -344,6 +415,13 @@ struct TcMap {  // shared memory, bytes from a 1024-byte boundary
   static constexpr int kRaw = (kBad + 2 * 8 * (int)sizeof(Cleared) + 127) / 128 * 128;
 };
 
+// Eight floats as one 32-byte sector: two 16-byte halves would each make L2 fetch the rest of it from memory.
+__device__ __forceinline__ void store_sector(float* p, const float* v) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]),
+               "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
+
 // Bounded mbarrier wait: about half a second of polls, far above any pipeline stage.
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
   for (int i = 0; i < (1 << 16); ++i) {
@@ -374,6 +452,14 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// D[tmem] (+)= A·B of kind::f16, the two shared-memory descriptors given by their lower words and the common upper one.
+__device__ __forceinline__ void mma_words(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 da, db;\n mov.b64 da, {%1, %3};\n mov.b64 db, {%2, %3};\n"
+      " setp.ne.b32 p, %5, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n}\n" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
 }
 // Any of the two 16-bit values of w is an infinity or NaN.
 template <typename T>
@@ -437,11 +523,11 @@ __device__ __forceinline__ uint4 dequant8(uint32_t w0, uint32_t w1, T sc, T bi) 
 }
 
 // Adds Σ p_j·v_j over the cleared drafted rows j that packed row pr (tree row t) sees to half `grp` of its output
-// (yrow, normalised by inv) or partial (orow), read from the cache. Their V holds an infinity or NaN, so this
+// (yrow, normalised by inv) or partial (slot, row), read from the cache. Their V holds an infinity or NaN, so this
 // runs for broken inputs only; the finite channels of such an output row are rounded once more per row added.
 template <typename T, int D, int BITS>
 __device__ __forceinline__ void add_cleared(const TreeArgs& a, int b, int g, const Cleared* bad, int seg, int pr, int t,
-                                            int ctx, float m_ref, float inv, int grp, T* yrow, float* orow) {
+                                            int ctx, float m_ref, float inv, int grp, T* yrow, int slot, int row) {
   const T* q = static_cast<const T*>(a.q) + (((int64_t)b * a.HKV + g) * a.R + pr) * D;
 #pragma unroll 1
   for (int j = 0; j < a.T; ++j) {
@@ -464,8 +550,12 @@ __device__ __forceinline__ void add_cleared(const TreeArgs& a, int b, int g, con
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int c = grp * D + c8 * 8 + e;
-        if (yrow) yrow[c] = from_f<T>(fmaf(p * inv, v[e], to_f<T>(yrow[c])));
-        else orow[c] = fmaf(p, v[e], orow[c]);
+        if (yrow) {
+          yrow[c] = from_f<T>(fmaf(p * inv, v[e], to_f<T>(yrow[c])));
+        } else {
+          float& o = a.part_o[part_at<D>(a, slot, c >> 3, row) + e];
+          o = fmaf(p, v[e], o);
+        }
       }
     }
   }
@@ -501,6 +591,35 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   pdl_trigger();
+  Schedule sched(a);
+  Segment sg;
+  bool more = sched.next(a, sg);
+  const bool softmax = warp >= 2 && warp < 10;
+  const int grp = warp >= 6, q = warp & 3;  // softmax: a warp reads tensor-memory lanes 32·(warp mod 4) ..
+  const int r = q * 32 + lane;
+  // A query row's half (group A the first channels, B the second), issued before the first copies fill the memory
+  // system's queues: straight to its swizzled place, or (q4: the channels change places) through registers.
+  constexpr int kQRegs = BITS == 4 ? D / 16 : 1;
+  uint4 qv[kQRegs];
+  auto q_place = [&](int i) {
+    const int c8 = grp * (D / 16) + i;
+    return Map::kQ + (c8 >> 3) * kTR * 128 + r * 128 + (((c8 & 7) ^ (r & 7)) << 4);
+  };
+  auto fetch_q = [&](const Segment& g) {
+    const int pr = g.rt * kTR + r;
+    const bool live = pr < a.R;
+    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) +
+                                                      (((int64_t)g.b * a.HKV + g.g) * a.R + (live ? pr : 0)) * D) + grp * (D / 16);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      if constexpr (BITS == 4)
+        qv[i] = live ? src[i] : make_uint4(0, 0, 0, 0);
+      else
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(sb + q_place(i)), "l"(src + i), "r"(live ? 16 : 0)
+                     : "memory");
+    }
+  };
+  if (softmax && more) fetch_q(sg);
   if (threadIdx.x == 0) {
     for (int i = 0; i < Map::kNumBars; ++i) {
       int count = 1;
@@ -524,14 +643,12 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
   tc::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  Schedule sched(a);
-  Segment sg;
   // Below, `it` counts this CTA's key tiles over all its segments: ring stages and barrier parities follow it.
   if (warp == 0) {
     if (lane == 0) {  // ---- copies ----
       int it = 0, k_iss = 0, v_iss = 0;
       bool ok = true;
-      while (ok && next_segment(a, sched, sg)) {
+      for (; ok && more; more = sched.next(a, sg)) {
         for (int kt = sg.t0; kt < sg.t1; ++kt, ++it) {
           const int p0 = kt * kTK;
           if (*abort_flag) { ok = false; break; }
@@ -582,75 +699,76 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
       for (int j = max(0, v_iss - ring); j < v_iss; ++j)
         if (!bar_wait(v_full(j % ring), (j / ring) & 1)) *abort_flag = 1;
     }
-  } else if (warp == 1) {
-    if (lane == 0) {  // ---- MMAs ----
-      constexpr uint32_t idesc_qk = tc::idesc_f16_f32(kTR, kTK, false, false, kBf16);
-      constexpr uint32_t idesc_pv = tc::idesc_f16_f32(kTR, 2 * D, true, false, kBf16);
-      auto issue_qk = [&](int it) -> bool {
-        const int s = it % NS;
-        if (!bar_wait(k_full(s), (it / NS) & 1)) return false;
-        tc::tc_fence_after();
-        const uint32_t kb = sb + Map::kK + s * Map::kKBytes;
+  } else if (warp == 1) {  // ---- MMAs: the warp walks the tiles together, one lane issues ----
+    constexpr uint32_t idesc_qk = tc::idesc_f16_f32(kTR, kTK, false, false, kBf16);
+    constexpr uint32_t idesc_pv = tc::idesc_f16_f32(kTR, 2 * D, true, false, kBf16);
+    // Descriptors as words: the upper ones are constants and the lower ones advance by constants, so that the
+    // issuing lane has one addition per product.
+    constexpr uint64_t kd = 1024 >> 4 | 1u << 14 | 2u << 29;  // K-major and MN-major alike: 1024-byte atoms, 128-byte swizzle
+    constexpr uint32_t hi = (uint32_t)kd;
+    const uint32_t q_lo = ((sb + Map::kQ) >> 4) | 1u << 16, k_lo = ((sb + Map::kK) >> 4) | 1u << 16;
+    const uint32_t p_lo = ((sb + Map::kP) >> 4) | 1u << 16, v_lo = ((sb + Map::kV) >> 4) | (kTK * 128 >> 4) << 16;
+    const bool leader = lane == 0;
+    auto issue_qk = [&](int it) -> bool {
+      const int s = it % NS;
+      if (!bar_wait(k_full(s), (it / NS) & 1)) return false;
+      tc::tc_fence_after();
+      if (leader) {
+        const uint32_t kl = k_lo + s * (Map::kKBytes >> 4), d = tmem + kColS + 64 * (it & 1);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          tc::mma_f16(tmem + kColS + 64 * (it & 1),
-                      tc::desc_kmajor_sw128(sb + Map::kQ + (kk >> 2) * kTR * 128 + (kk & 3) * 32),
-                      tc::desc_kmajor_sw128(kb + (kk >> 2) * kTK * 128 + (kk & 3) * 32), idesc_qk, kk > 0);
+          mma_words(d, q_lo + (kk >> 2) * (kTR * 128 >> 4) + (kk & 3) * 2, kl + (kk >> 2) * (kTK * 128 >> 4) + (kk & 3) * 2, hi,
+                    idesc_qk, kk > 0);
         tc::mma_commit(s_full(it & 1));
         tc::mma_commit(k_empty(s));
-        return true;
-      };
-      int it = 0, seg = 0;
-      bool ok = true;
-      for (; ok && next_segment(a, sched, sg); ++seg) {
-        ok = bar_wait(q_full, seg & 1) && issue_qk(it);
-        for (int kt = sg.t0; ok && kt < sg.t1; ++kt, ++it) {
-          if (*abort_flag || (kt + 1 < sg.t1 && !issue_qk(it + 1))) { ok = false; break; }
-          const int s = it % NS;
-          if (!bar_wait(p_full(it & 1), (it >> 1) & 1) || !bar_wait(v_full(s), (it / NS) & 1)) {
-            ok = false;
-            break;
-          }
-          tc::tc_fence_after();
-          const uint32_t pb = sb + Map::kP + (it & 1) * kTR * 128, vb = sb + Map::kV + s * Map::kVBytes;
+      }
+      __syncwarp();
+      return true;
+    };
+    int it = 0, seg = 0;
+    bool ok = true;
+    for (; ok && more; more = sched.next(a, sg), ++seg) {
+      ok = bar_wait(q_full, seg & 1) && issue_qk(it);
+      for (int kt = sg.t0; ok && kt < sg.t1; ++kt, ++it) {
+        if (*abort_flag || (kt + 1 < sg.t1 && !issue_qk(it + 1))) { ok = false; break; }
+        const int s = it % NS;
+        if (!bar_wait(p_full(it & 1), (it >> 1) & 1) || !bar_wait(v_full(s), (it / NS) & 1)) { ok = false; break; }
+        tc::tc_fence_after();
+        if (leader) {
+          const uint32_t pl = p_lo + (it & 1) * (kTR * 128 >> 4), vl = v_lo + s * (Map::kVBytes >> 4);
 #pragma unroll
           for (int kk = 0; kk < kTK / 16; ++kk)
-            tc::mma_f16(tmem + kColO, tc::desc_kmajor_sw128(pb + kk * 32),
-                        tc::desc_mnmajor_sw128(vb + kk * 2048, kTK * 128, 1024), idesc_pv, kt > sg.t0 || kk > 0);
+            mma_words(tmem + kColO, pl + kk * 2, vl + kk * (2048 >> 4), hi, idesc_pv, kt > sg.t0 || kk > 0);
           tc::mma_commit(o_done(it & 1));
           tc::mma_commit(v_empty(s));
         }
+        __syncwarp();
       }
-      if (!ok) *abort_flag = 1;
-      // every MMA this thread issued completes before tensor memory can be freed
-      tc::mma_commit(drain);
-      if (!bar_wait(drain, 0)) *abort_flag = 1;
+      ok = __all_sync(0xffffffffu, ok);
     }
+    if (!ok) *abort_flag = 1;
+    // every MMA this warp issued completes before tensor memory can be freed
+    if (leader) tc::mma_commit(drain);
     __syncwarp();
+    if (!bar_wait(drain, 0)) *abort_flag = 1;
   } else if (warp < 10) {  // ---- softmax: one thread per query row, two groups ----
-    const int grp = warp >= 6, q = warp & 3;  // a warp reads tensor-memory lanes 32·(warp mod 4) ..
-    const int r = q * 32 + lane;
     const uint32_t trow = tmem + ((uint32_t)(q * 32) << 16);
     const float mult = fabsf(a.scale_log2);
+    const uint32_t flip = a.scale_log2 < 0.f ? 0x80000000u : 0u;  // scale < 0: −S with |scale|
     float* m_row = reinterpret_cast<float*>(smem + Map::kState) + r;
     float* l_row = m_row + kTR;  // group g's sum at l_row[g * kTR]
     Cleared* bad_all = reinterpret_cast<Cleared*>(smem + Map::kBad);
-    auto load_q = [&](const Segment& g) {  // group A the first half of the channels, B the second
-      const int pr = g.rt * kTR + r;
-      const T* src = static_cast<const T*>(a.q) + (((int64_t)g.b * a.HKV + g.g) * a.R + pr) * D;
-      const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;  // scale < 0: −q with |scale|
+    auto store_q = [&]() {
+      if constexpr (BITS == 4) {
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const int c8 = grp * (D / 16) + i;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (pr < a.R) {
-          v = *reinterpret_cast<const uint4*>(src + c8 * 8);
-          if constexpr (BITS == 4)  // (0,1)(2,3)(4,5)(6,7) -> (0,4)(1,5)(2,6)(3,7)
-            v = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
-                           __byte_perm(v.y, v.w, 0x7632));
-          v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
+        for (int i = 0; i < D / 16; ++i) {  // (0,1)(2,3)(4,5)(6,7) -> (0,4)(1,5)(2,6)(3,7)
+          const uint4 v = qv[i];
+          *reinterpret_cast<uint4*>(smem + q_place(i)) =
+              make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
+                         __byte_perm(v.y, v.w, 0x7632));
         }
-        *reinterpret_cast<uint4*>(smem + Map::kQ + (c8 >> 3) * kTR * 128 + r * 128 + (((c8 & 7) ^ (r & 7)) << 4)) = v;
+      } else {
+        asm volatile("cp.async.wait_all;\n" ::: "memory");
       }
       tc::fence_proxy_async_smem();
       __syncwarp();
@@ -664,23 +782,21 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
     bool alive = true;
     int it = 0, seg = 0;
     int handed = 0, joined = 0;  // phases of m_next and l_both: a warp without a row takes no part in a segment's
-    Segment nx;
-    bool more = next_segment(a, sched, nx);
-    if (more) load_q(nx);
+    if (more) store_q();
     while (more) {
-      sg = nx;
       const int pr = sg.rt * kTR + r;
       const bool live = pr < a.R;
       const bool work = sg.rt * kTR + q * 32 < a.R;  // this warp has a row
       const int t = live ? pr % a.T : 0;
       const int ctx = sg.n - a.T;
+      // read before the first tile arrives
+      const uint64_t mrow = live && a.T <= 64 && sg.t1 * kTK > ctx ? mask_bits(a, sg.b, t, 0) : 0;
       float m_mine = -INFINITY, l = 0.f;  // the maximum that l refers to
       for (int kt = sg.t0; kt < sg.t1; ++kt, ++it) {
         if ((it & 1) != grp || !alive) continue;
         const int p0 = kt * kTK;
         const bool tail = p0 + kTK > ctx;  // drafted rows or the cache's end in this tile
-        uint64_t vis = 0;
-        if (tail && live) vis = visible<kTK>(a, sg.b, t, sg.n, p0);
+        const uint64_t vis = tail && live ? visible(a, mrow, sg.b, t, ctx, p0) : 0;
         if (!(alive = wait(s_full(grp), it >> 1))) continue;
         tc::tc_fence_after();
         const uint32_t ts = trow + kColS + 64 * grp;
@@ -693,6 +809,10 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
           uint32_t u[32];
           tc::tmem_ld32(ts + 32 * h, u);
           tc::tmem_ld_wait();
+          if (flip) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) u[c] ^= flip;
+          }
           if (tail) {
             const uint32_t v = (uint32_t)(vis >> (32 * h));
 #pragma unroll
@@ -808,11 +928,16 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(p_full(grp));
       }
-      more = next_segment(a, sched, nx);
+      Segment nx;
+      more = sched.next(a, nx);
+      if (BITS == 4 && more) fetch_q(nx);
       const int e = it - 1;  // the segment's last tile
       if (alive) alive = wait(s_full(e & 1), e >> 1);
       // its S is complete: Q is free, and the next segment's first product can start
-      if (more && alive) load_q(nx);
+      if (more && alive) {
+        if (BITS != 4) fetch_q(nx);
+        store_q();
+      }
       if (alive) alive = wait(o_done(e & 1), e >> 1);
       tc::tc_fence_after();
       if (work) {
@@ -826,72 +951,43 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
           alive = wait(l_both(q), joined++);
           l = l_row[0] + l_row[kTR];
         }
-        // Through this warp's 4 KB of its group's P buffer: its last P·V is complete.
         const float inv = !alive ? NAN : l == 0.f ? 0.f : 1.f / l;
-        uint8_t* stage = smem + Map::kP + grp * kTR * 128 + q * 32 * 128;
-        const int64_t row0 = ((int64_t)sg.b * a.HKV + sg.g) * a.R + sg.rt * kTR + q * 32;  // first of the warp's rows
-        const int rows = min(32, a.R - (sg.rt * kTR + q * 32));
+        const int64_t row = ((int64_t)sg.b * a.HKV + sg.g) * a.R + pr;
         const Cleared* bad = bad_all + (seg & 1) * 8;
         bool any_bad = false;
 #pragma unroll
         for (int w = 0; w < 8; ++w) any_bad |= bad[w].seg == seg;
-        if (sg.slot >= 0 && live && grp == 0) {
-          float* ml = a.part_ml + ((int64_t)sg.slot * a.slot_rows + r) * 2;
-          ml[0] = m_ref;
-          ml[1] = alive ? l : NAN;
-        }
-        const int cb0 = grp * (D / 32);
-        {
+        if (sg.slot >= 0 && live && grp == 0)
+          *reinterpret_cast<float2*>(a.part_ml + ((int64_t)sg.slot * a.slot_rows + r) * 2) = make_float2(m_ref, alive ? l : NAN);
+        // a thread writes whole 32-byte sectors of its row
 #pragma unroll 1
-          for (int cb = cb0; cb < cb0 + D / 32; ++cb) {
-            uint32_t ov[32];
-            tc::tmem_ld32(trow + kColO + cb * 32, ov);
-            tc::tmem_ld_wait();
-            float o[32];
+        for (int cb = grp * (D / 32); cb < (grp + 1) * (D / 32); ++cb) {
+          uint32_t ov[32];
+          tc::tmem_ld32(trow + kColO + cb * 32, ov);
+          tc::tmem_ld_wait();
+          if (!live) continue;
+          float o[32];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[(i & ~7) + chunk_channel<BITS>(i & 7)] = alive ? __uint_as_float(ov[i]) : NAN;
-            if (sg.slot < 0) {  // 32 rows × 64 bytes
+          for (int i = 0; i < 32; ++i) o[(i & ~7) + chunk_channel<BITS>(i & 7)] = alive ? __uint_as_float(ov[i]) : NAN;
+          if (sg.slot < 0) {
+            T* dst = static_cast<T*>(a.y) + row * 2 * D + cb * 32;
 #pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                uint4 v;
-                v.x = pack2<T>(o[8 * c] * inv, o[8 * c + 1] * inv);
-                v.y = pack2<T>(o[8 * c + 2] * inv, o[8 * c + 3] * inv);
-                v.z = pack2<T>(o[8 * c + 4] * inv, o[8 * c + 5] * inv);
-                v.w = pack2<T>(o[8 * c + 6] * inv, o[8 * c + 7] * inv);
-                *reinterpret_cast<uint4*>(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = v;
-              }
-              __syncwarp();
+            for (int c = 0; c < 4; ++c)
+              *reinterpret_cast<uint4*>(dst + 8 * c) =
+                  make_uint4(pack2<T>(o[8 * c] * inv, o[8 * c + 1] * inv), pack2<T>(o[8 * c + 2] * inv, o[8 * c + 3] * inv),
+                             pack2<T>(o[8 * c + 4] * inv, o[8 * c + 5] * inv), pack2<T>(o[8 * c + 6] * inv, o[8 * c + 7] * inv));
+          } else {
+            float* dst = a.part_o + part_at<D>(a, sg.slot, cb * 4, r);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int rr = i * 8 + (lane >> 2), c = lane & 3;
-                const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 64 + ((c ^ ((rr >> 1) & 3)) << 4));
-                if (rr < rows)
-                  *reinterpret_cast<uint4*>(static_cast<T*>(a.y) + (row0 + rr) * 2 * D + cb * 32 + c * 8) = v;
-              }
-            } else {  // 32 rows × 128 bytes
-#pragma unroll
-              for (int c = 0; c < 8; ++c)
-                *reinterpret_cast<float4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) =
-                    make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
-              __syncwarp();
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const int rr = i * 4 + (lane >> 3), c = lane & 7;
-                const float4 v = *reinterpret_cast<const float4*>(stage + rr * 128 + ((c ^ (rr & 7)) << 4));
-                if (rr < rows)
-                  *reinterpret_cast<float4*>(a.part_o + ((int64_t)sg.slot * a.slot_rows + q * 32 + rr) * 2 * D + cb * 32 +
-                                             c * 4) = v;
-              }
-            }
-            __syncwarp();
+            for (int c = 0; c < 4; ++c) store_sector(dst + (int64_t)c * a.slot_rows * 8, o + 8 * c);
           }
         }
         if (any_bad && alive && live)
           add_cleared<T, D, BITS>(a, sg.b, sg.g, bad, seg, pr, t, ctx, m_ref, inv, grp,
-                                  sg.slot < 0 ? static_cast<T*>(a.y) + (row0 + lane) * 2 * D : nullptr,
-                                  a.part_o + ((int64_t)max(sg.slot, 0) * a.slot_rows + r) * 2 * D);
+                                  sg.slot < 0 ? static_cast<T*>(a.y) + row * 2 * D : nullptr, sg.slot, r);
       }
       if (!alive) *abort_flag = 1;
+      sg = nx;
       ++seg;
     }
   } else if constexpr (BITS != 16) {  // ---- operand tiles from packed rows ----
@@ -900,7 +996,7 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
     constexpr int kUnits = kTK * D / 32;  // 32 channels of one row
     int it = 0;
     bool alive = true;
-    while (alive && next_segment(a, sched, sg)) {
+    for (; alive && more; more = sched.next(a, sg)) {
       for (int kt = sg.t0; kt < sg.t1; ++kt, ++it) {
         const int rs = it % ta.raw_stages, s = it % NS;
         const uint32_t par = (it / NS - 1) & 1;
@@ -958,93 +1054,120 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
 }
 
 // ---- join of the cut units' partials -----------------------------------------------------------------
-// One warp per output row: O = Σ w·O_s / Σ w·l_s, w = 2^(m_s − max m), over the CTAs that held a part
-// of the row's unit, in their order. `grid` is the attention kernel's.
+// O = Σ w·O_s / Σ w·l_s, w = 2^(m_s − max m), over the parts of the row's unit in their order. Four warps
+// take every fourth part of one output row and add up through shared memory; a lane holds eight channels
+// (one sector of a part; D 64: two parts at a time).
+constexpr int kMergeWarps = 4, kMergeRows = 2;
+
 template <typename T, int D>
-__global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__ TreeArgs a, int grid) {
-  constexpr int V = 2 * D / 32;  // channels of a lane: two (D 128: four) groups of 4, 128 apart
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int64_t rows_b = (int64_t)a.HKV * a.R;
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  if (row >= a.B * rows_b) return;
-  const int b = (int)(row / rows_b);
-  const int pr = (int)(row % a.R), g = (int)(row % rows_b / a.R);
+__global__ void __launch_bounds__(32 * kMergeWarps * kMergeRows) tree_merge_kernel(const __grid_constant__ TreeArgs a, int grid) {
+  constexpr int kChunks = 2 * D / 8;         // lanes of one part
+  constexpr int kSub = 32 / kChunks;         // parts of one warp step
+  constexpr int kStep = kMergeWarps * kSub;  // parts of one step of the row's warps
+  __shared__ __align__(16) float so[kMergeRows][kStep][2 * D];
+  __shared__ float2 sml[kMergeRows][kStep];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int slot_row = warp / kMergeWarps, w = warp % kMergeWarps;
+  const int64_t row = (int64_t)blockIdx.x * kMergeRows + slot_row;
+  const int rows_b = a.HKV * a.R;
+  const bool valid = row < (int64_t)a.B * rows_b;
+  const int b = valid ? (int)(row / rows_b) : 0, in_b = valid ? (int)(row - (int64_t)b * rows_b) : 0;
+  const int g = in_b / a.R, pr = in_b - g * a.R;
   const int rt = pr / a.tile_rows, r = pr - rt * a.tile_rows;
-  const int per_b = a.HKV * a.row_tiles;
-  int64_t total = 0, base = 0;
-  for (int i = lane; i < a.B; i += 32) {
-    const int nt = key_tiles(a, live_rows(a, i));
-    total += nt;
-    base += i < b ? nt : 0;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    total += __shfl_xor_sync(0xffffffffu, total, o);
-    base += __shfl_xor_sync(0xffffffffu, base, o);
-  }
-  total *= per_b;
+  const int per_b = a.HKV * a.row_tiles, u = g * a.row_tiles + rt;
+  // parts first .. first + parts − 1 of the unit; part k's place, -1 for an empty one
+  int parts, first = 0, at = 0;
+  Line line;
   const int nt = key_tiles(a, live_rows(a, b));
-  const int64_t s = base * per_b + (int64_t)(g * a.row_tiles + rt) * nt, e = s + nt;
-  auto lo = [&](int64_t i) { return i * total / grid; };
-  const int64_t i0 = ((s + 1) * grid - 1) / total, i1 = (e * grid - 1) / total;  // CTAs of tiles s and e − 1
-  if (i0 == i1) return;  // written by its CTA
-  const int parts = (int)(i1 - i0) + 1;
-  // a lane holds one CTA's part at a time: its place, maximum and sum (an empty CTA has none)
-  auto part = [&](int k, int64_t& sr, float& m, float& l) {
-    m = -INFINITY, l = 0.f, sr = 0;
-    const int64_t i = i0 + k, at = lo(i);
-    if (k >= parts || at >= lo(i + 1)) return;
-    sr = (2 * i + (at >= s ? 0 : 1)) * a.slot_rows + r;
-    const float2 f = *reinterpret_cast<const float2*>(a.part_ml + sr * 2);
-    m = f.x, l = f.y;
-  };
-  int64_t sr;
-  float m, l, M = -INFINITY;
-  for (int k0 = 0; k0 < parts; k0 += 32) {
-    part(k0 + lane, sr, m, l);
-    M = fmaxf(M, m);
+  if (a.cuts) {
+    parts = nt > 1 ? a.cuts : 1;
+    first = (b * per_b + u) * a.cuts;
+  } else {
+    int tiles = 0, before = 0;
+    for (int i = lane; i < a.B; i += 32) {
+      const int x = key_tiles(a, live_rows(a, i));
+      tiles += x;
+      before += i < b ? x : 0;
+    }
+    tiles = (int)__reduce_add_sync(0xffffffffu, (unsigned)tiles) * per_b;
+    before = (int)__reduce_add_sync(0xffffffffu, (unsigned)before) * per_b;
+    line.init(tiles, a.B * per_b, grid);
+    at = before + b * per_b * line.lead + u * (nt + line.lead) + line.lead;  // the unit's first key tile
+    first = line.owner(at);
+    parts = line.owner(at + nt - 1) - first + 1;
   }
-  M = warp_max(M);
-  float L = 0.f, o[V] = {};
-  for (int k0 = 0; k0 < parts; k0 += 32) {
-    if (parts > 32 || k0 > 0) part(k0 + lane, sr, m, l);
-    const float w = m == -INFINITY ? 0.f : exp2f(m - M);
-    L += w == 0.f ? 0.f : w * l;
-    const int nk = min(32, parts - k0);
-    constexpr int kU = 4;  // parts in flight
-    for (int k = 0; k < nk; k += kU) {
-      float4 f[kU][V / 4];
-      float wk[kU];
+  auto place = [&](int k) -> int {
+    if (a.cuts) return cut_at(k, nt, a.cuts) < cut_at(k + 1, nt, a.cuts) ? first + k : -1;
+    const int from = line.lo(first + k);
+    return from >= line.lo(first + k + 1) ? -1 : 2 * (first + k) + (from > at ? 0 : 1);
+  };
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");  // every thread: the launch ends after the one before it
+  const bool join = valid && parts > 1;                  // else written by its CTA
+  const int sub = lane / kChunks, chunk = lane % kChunks;
+  float M = -INFINITY, L = 0.f, o[8] = {};
+  if (join) {
+    constexpr int kU = 5;  // parts in flight
+    for (int k0 = w * kSub + sub; k0 < parts; k0 += kStep * kU) {
+      float m[kU], l[kU];
+      float4 f[kU][2];
 #pragma unroll
       for (int x = 0; x < kU; ++x) {
-        const int kk = min(k + x, nk - 1);
-        wk[x] = __shfl_sync(0xffffffffu, w, kk);
-        const int64_t srk = __shfl_sync(0xffffffffu, sr, kk);
-        if (k + x >= nk) wk[x] = 0.f;
-        if (wk[x] == 0.f) continue;
-#pragma unroll
-        for (int v = 0; v < V / 4; ++v) f[x][v] = reinterpret_cast<const float4*>(a.part_o + srk * 2 * D)[v * 32 + lane];
+        const int k = k0 + x * kStep, at_ = k < parts ? place(k) : -1;
+        m[x] = -INFINITY, l[x] = 0.f;
+        if (at_ < 0) continue;
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + ((int64_t)at_ * a.slot_rows + r) * 2);
+        const float4* p = reinterpret_cast<const float4*>(a.part_o + part_at<D>(a, at_, chunk, r));
+        m[x] = ml.x, l[x] = ml.y;
+        f[x][0] = p[0], f[x][1] = p[1];
       }
+      float top = M;
+#pragma unroll
+      for (int x = 0; x < kU; ++x) top = fmaxf(top, m[x]);
+      const float c0 = top == M ? 1.f : exp2f(M - top);
+      M = top, L *= c0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] *= c0;
 #pragma unroll
       for (int x = 0; x < kU; ++x) {
-        if (wk[x] == 0.f) continue;  // a part that saw no key of this row
-#pragma unroll
-        for (int v = 0; v < V / 4; ++v) {
-          o[4 * v] = fmaf(wk[x], f[x][v].x, o[4 * v]);
-          o[4 * v + 1] = fmaf(wk[x], f[x][v].y, o[4 * v + 1]);
-          o[4 * v + 2] = fmaf(wk[x], f[x][v].z, o[4 * v + 2]);
-          o[4 * v + 3] = fmaf(wk[x], f[x][v].w, o[4 * v + 3]);
+        if (m[x] == -INFINITY) {  // empty, or a part that saw no key of this row: its O is not used
+          L += l[x] == l[x] ? 0.f : l[x];
+          continue;
         }
+        const float c = exp2f(m[x] - M);
+        L = fmaf(c, l[x], L);
+        o[0] = fmaf(c, f[x][0].x, o[0]), o[1] = fmaf(c, f[x][0].y, o[1]);
+        o[2] = fmaf(c, f[x][0].z, o[2]), o[3] = fmaf(c, f[x][0].w, o[3]);
+        o[4] = fmaf(c, f[x][1].x, o[4]), o[5] = fmaf(c, f[x][1].y, o[5]);
+        o[6] = fmaf(c, f[x][1].z, o[6]), o[7] = fmaf(c, f[x][1].w, o[7]);
       }
     }
+    const int ps = w * kSub + sub;
+    reinterpret_cast<float4*>(&so[slot_row][ps][chunk * 8])[0] = make_float4(o[0], o[1], o[2], o[3]);
+    reinterpret_cast<float4*>(&so[slot_row][ps][chunk * 8])[1] = make_float4(o[4], o[5], o[6], o[7]);
+    if (chunk == 0) sml[slot_row][ps] = make_float2(M, L);
   }
-  L = warp_sum(L);
-  const float inv = L == 0.f ? 0.f : 1.f / L;
+  __syncthreads();
+  if (!join) return;
+  float top = -INFINITY, den = 0.f, c[kStep];
 #pragma unroll
-  for (int v = 0; v < V / 4; ++v) {
-    const float f[4] = {o[4 * v] * inv, o[4 * v + 1] * inv, o[4 * v + 2] * inv, o[4 * v + 3] * inv};
-    store_vec<T, 4>(static_cast<T*>(a.y) + row * 2 * D + (v * 32 + lane) * 4, f);
+  for (int i = 0; i < kStep; ++i) top = fmaxf(top, sml[slot_row][i].x);
+#pragma unroll
+  for (int i = 0; i < kStep; ++i) {
+    const float2 ml = sml[slot_row][i];
+    c[i] = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
+    den += ml.x == -INFINITY ? ml.y : c[i] * ml.y;
+  }
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+  for (int ch = threadIdx.x % (32 * kMergeWarps); ch < D; ch += 32 * kMergeWarps) {  // two channels a thread
+    float2 v = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < kStep; ++i) {
+      if (c[i] == 0.f) continue;
+      const float2 p = *reinterpret_cast<const float2*>(&so[slot_row][i][2 * ch]);
+      v.x = fmaf(c[i], p.x, v.x), v.y = fmaf(c[i], p.y, v.y);
+    }
+    T* dst = static_cast<T*>(a.y) + row * 2 * D + 2 * ch;
+    dst[0] = from_f<T>(v.x * inv), dst[1] = from_f<T>(v.y * inv);
   }
 }
 
@@ -1061,14 +1184,18 @@ constexpr int64_t kMaxTreeRows = 256;
 struct Plan {
   bool tc;
   int tile_rows, tile_keys, row_tiles, slot_rows;
+  int cuts;       // parts of every unit, or 0: the line
   int64_t tiles;  // key tiles of all units at the longest lengths
-  int64_t grid;   // at most the CTAs that run at once, and one per tile
+  int64_t grid;   // CTAs: at most as many as run at once
   size_t ml_offset, bytes;
 };
 
 // The tensor-core form takes 16-bit types; packed rows need tiles that start on 16-byte boundaries in the
 // scales too (any capacity that is a multiple of 8 does). The rest runs on the CUDA cores.
-Plan make_plan(int dtype, int bits, int gs, int64_t B, int64_t HKV, int64_t R, int64_t D, int64_t cap, int64_t len_bound) {
+// Units of one length are cut evenly where that uses most of the CTAs that run at once; more parts than
+// √(6·tiles) cost more in the join than they save.
+Plan make_plan(int dtype, int bits, int gs, int64_t B, int64_t HKV, int64_t R, int64_t D, int64_t cap, int64_t len_bound,
+               bool one_length) {
   Plan p{};
   p.tc = dtype != MOTIF_F32 && (bits == 16 || (cap * (D / gs)) % 8 == 0);
   p.tile_rows = p.tc ? kTR : kSR;
@@ -1076,41 +1203,57 @@ Plan make_plan(int dtype, int bits, int gs, int64_t B, int64_t HKV, int64_t R, i
   p.row_tiles = (int)ceil_div(R, p.tile_rows);
   p.slot_rows = (int)(R < p.tile_rows ? R : p.tile_rows);
   const int64_t ctas = (p.tc ? 1 : 2) * (int64_t)sm_count();
-  p.tiles = ceil_div(len_bound < 1 ? 1 : len_bound, p.tile_keys) * B * HKV * p.row_tiles;
+  const int64_t nt = ceil_div(len_bound < 1 ? 1 : len_bound, p.tile_keys), units = B * HKV * p.row_tiles;
+  p.tiles = nt * units;
   p.grid = p.tiles < ctas ? p.tiles : ctas;
-  p.ml_offset = sizeof(float) * 2 * (size_t)p.grid * p.slot_rows * 2 * (size_t)D;
-  p.bytes = p.ml_offset + sizeof(float) * 2 * (size_t)p.grid * p.slot_rows * 2;
+  int64_t parts = 2 * p.grid;
+  if ((one_length || B == 1) && units <= ctas && B < 65536 && HKV * p.row_tiles < 65536) {
+    int64_t c = ctas / units;
+    if (c > nt) c = nt;
+    while (c > 1 && c * c > 6 * nt) --c;
+    if (c == nt || c < ctas / units || 8 * c * units >= 7 * ctas) {
+      p.cuts = (int)c;
+      parts = c * units;
+    }
+  }
+  p.ml_offset = sizeof(float) * (size_t)parts * p.slot_rows * 2 * (size_t)D;
+  p.bytes = p.ml_offset + sizeof(float) * (size_t)parts * p.slot_rows * 2;
   return p;
 }
 
+dim3 grid_of(const TreeArgs& a, const Plan& p) {
+  return a.cuts ? dim3((unsigned)a.cuts, (unsigned)(a.HKV * a.row_tiles), (unsigned)a.B) : dim3((unsigned)p.grid);
+}
+
 template <typename T, int D>
-int launch_merge(const TreeArgs& a, int64_t grid, cudaStream_t st) {
+int launch_merge(const TreeArgs& a, const Plan& p, cudaStream_t st) {
+  if (a.cuts == 1) return MOTIF_OK;  // every unit in one part
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)ceil_div((int64_t)a.B * a.HKV * a.R, 8));
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3((unsigned)ceil_div((int64_t)a.B * a.HKV * a.R, kMergeRows));
+  cfg.blockDim = dim3(32 * kMergeWarps * kMergeRows);
   cfg.stream = st;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, tree_merge_kernel<T, D>, a, (int)grid);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, tree_merge_kernel<T, D>, a, (int)p.grid);
   if (e != cudaSuccess) return fail(MOTIF_ERR_CUDA, "sdpa_dual_v_tree: merge launch: %s", cudaGetErrorString(e));
   return MOTIF_OK;
 }
 
 template <typename T, int D, int BITS>
-int launch_simt(TreeArgs& a, int64_t grid, cudaStream_t st) {
+int launch_simt(const TreeArgs& a, const Plan& p, cudaStream_t st) {
   auto kern = tree_simt_kernel<T, D, BITS>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, simt_smem<D>());
   if (e != cudaSuccess) return fail(MOTIF_ERR_CUDA, "sdpa_dual_v_tree: smem attribute: %s", cudaGetErrorString(e));
-  kern<<<(unsigned)grid, kSThreads, simt_smem<D>(), st>>>(a);
+  kern<<<grid_of(a, p), kSThreads, simt_smem<D>(), st>>>(a);
   const int rc = check_launch("sdpa_dual_v_tree");
-  return rc ? rc : launch_merge<T, D>(a, grid, st);
+  return rc ? rc : launch_merge<T, D>(a, p, st);
 }
 
 template <typename T, int D, int BITS>
-int launch_tc(const TreeArgs& a, int64_t grid, cudaStream_t st) {
+int launch_tc(const TreeArgs& a, const Plan& p, cudaStream_t st) {
   using Map = TcMap<D, BITS>;
   TcArgs ta{};
   ta.t = a;
@@ -1133,16 +1276,16 @@ int launch_tc(const TreeArgs& a, int64_t grid, cudaStream_t st) {
   auto kern = tree_tc_kernel<T, D, BITS>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return fail(MOTIF_ERR_CUDA, "sdpa_dual_v_tree: smem attribute: %s", cudaGetErrorString(e));
-  kern<<<(unsigned)grid, TcCfg<BITS>::kThreads, smem, st>>>(ta);
+  kern<<<grid_of(a, p), TcCfg<BITS>::kThreads, smem, st>>>(ta);
   const int rc = check_launch("sdpa_dual_v_tree");
-  return rc ? rc : launch_merge<T, D>(a, grid, st);
+  return rc ? rc : launch_merge<T, D>(a, p, st);
 }
 
 template <typename T, int D, int BITS>
-int launch(TreeArgs& a, const Plan& p, cudaStream_t st) {
+int launch(const TreeArgs& a, const Plan& p, cudaStream_t st) {
   if constexpr (!std::is_same<T, float>::value)
-    if (p.tc) return launch_tc<T, D, BITS>(a, p.grid, st);
-  return launch_simt<T, D, BITS>(a, p.grid, st);
+    if (p.tc) return launch_tc<T, D, BITS>(a, p, st);
+  return launch_simt<T, D, BITS>(a, p, st);
 }
 
 }  // namespace
@@ -1154,11 +1297,12 @@ extern "C" {
 
 size_t motif_sdpa_dual_v_tree_workspace_bytes(int dtype, int bits, int group_size, int64_t batch, int64_t h_q,
                                               int64_t h_kv, int64_t tree_rows, int64_t kv_cap, int64_t head_dim,
-                                              int64_t kv_len_bound) {
+                                              int64_t kv_len_bound, int one_length) {
   if (batch < 1 || h_q < 1 || h_kv < 1 || tree_rows < 1 || kv_cap < 1 || head_dim < 1 || group_size < 1 ||
       head_dim < group_size)
     return 0;
-  return make_plan(dtype, bits, group_size, batch, h_kv, h_q / h_kv * tree_rows, head_dim, kv_cap, kv_len_bound).bytes;
+  return make_plan(dtype, bits, group_size, batch, h_kv, h_q / h_kv * tree_rows, head_dim, kv_cap, kv_len_bound,
+                   one_length != 0).bytes;
 }
 
 int motif_sdpa_dual_v_tree(int dtype, int bits, int group_size, const void* q, const motif_tree_kv* kv,
@@ -1233,12 +1377,13 @@ int motif_sdpa_dual_v_tree(int dtype, int bits, int group_size, const void* q, c
   a.gs = group_size;
   a.scale_log2 = scale * kLog2e;
   const Plan p = make_plan(dtype, bits, bits == 16 ? 64 : group_size, batch, h_kv, a.R, head_dim, kv_cap,
-                           kv_len_dev ? kv_cap : kv_len);
+                           kv_len_dev ? kv_cap : kv_len, !kv_len_dev || kv_len_stride == 0);
   a.tile_rows = p.tile_rows;
   a.tile_keys = p.tile_keys;
   a.row_tiles = p.row_tiles;
   a.slot_rows = p.slot_rows;
-  MOTIF_REQUIRE(p.tiles < (1ll << 31) - 1, MOTIF_ERR_BAD_SHAPE, "sdpa_dual_v_tree: %lld key tiles in one call",
+  a.cuts = p.cuts;
+  MOTIF_REQUIRE(p.tiles < (1ll << 28), MOTIF_ERR_BAD_SHAPE, "sdpa_dual_v_tree: %lld key tiles in one call",
                 (long long)p.tiles);
   MOTIF_REQUIRE(workspace && workspace_bytes >= p.bytes, MOTIF_ERR_WORKSPACE,
                 "sdpa_dual_v_tree: workspace of %zu bytes, needs %zu", workspace_bytes, p.bytes);

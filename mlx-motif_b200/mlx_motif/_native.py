@@ -153,7 +153,7 @@ SIGNATURES = {
     "motif_argmax": (_I, [_I, _P, _L, _P, _P, _S, _P]),
     "motif_argmax_key_decode": (_I, [_P, _P, _P, _P]),
     "motif_argmax_key_exchange": (_I, [_P, _P, _I, _I, _P, _P, _P, _P, _P]),
-    "motif_sdpa_dual_v_tree_workspace_bytes": (_S, [_I, _I, _I, _L, _L, _L, _L, _L, _L, _L]),
+    "motif_sdpa_dual_v_tree_workspace_bytes": (_S, [_I, _I, _I, _L, _L, _L, _L, _L, _L, _L, _I]),
     "motif_sdpa_dual_v_tree": (
         _I,
         [_I, _I, _I, _P, _TKV, _P, _L, _F, _L, _L, _L, _L, _L, _L, _L, _P, _L, _P, _P, _S, _P, _P],

@@ -153,7 +153,7 @@ def _launch(q, parts, strides, bits, group_size, scale, HKV, cap, kv_len, tree_m
     with on_device(dev):
         qc = _aligned(q)
         ws_bytes = lib.motif_sdpa_dual_v_tree_workspace_bytes(code, bits, group_size, B, HQ, HKV, T, cap, D,
-                                                              cap if n_dev else n)
+                                                              cap if n_dev else n, 1 - n_step)
         ws = workspace(ws_bytes, dev)
         check(lib.motif_sdpa_dual_v_tree(code, bits, group_size, ptr(qc), C.byref(kv), ptr(mask), mask_b, float(scale),
                                          B, HQ, HKV, T, cap, D, n, n_dev, n_step, ptr(y), ptr(ws), ws_bytes, None,
