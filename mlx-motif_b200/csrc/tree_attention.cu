@@ -357,11 +357,12 @@ __global__ void __launch_bounds__(kSThreads, 2) tree_simt_kernel(const __grid_co
 // ---- tensor-core form: 16-bit rows and packed caches of 16-bit models --------------------------------
 // One CTA per SM takes 128 packed query rows (rows past the unit's are zero) and 64-key tiles:
 //   S = Q·Kᵀ (M 128, N 64, K D) and O += P·[V1 | V2] (M 128, N 2D, K 64) run as tcgen05.mma into tensor
-// memory (S double-buffered: 2 × 64 columns, O: 2D columns); Q, K and P are K-major, V is MN-major as the
-// cache rows lie, all in the 128-byte swizzle.
+// memory (S: kSBufs × 64 columns, O: 2D columns); Q and K are K-major and V is MN-major
+// as the cache rows lie, in the 128-byte swizzle; P replaces its S in tensor memory.
 //   warp 0       TMA: K and V tiles straight from the cache into rings of kStages (16-bit rows), or the
 //                packed rows, scales and biases into a ring of raw tiles;
-//   warp 1       one lane issues the MMAs, S one tile ahead within a segment;
+//   warp 1       one lane issues the MMAs, S up to kSBufs tiles ahead of P·V within a segment, so that the
+//                softmax groups find their tiles ready;
 //   warps 2..9   two softmax groups of four warps that take the tiles in turn (one warp alone on a
 //                scheduler waits out every latency of its 64-column row: tensor-memory reads, the maximum,
 //                the exponentials). A thread is a query row: it takes S from tensor memory and writes P in
@@ -382,11 +383,13 @@ constexpr int kTR = 128, kTK = 64;
 
 template <int BITS>
 struct TcCfg {
-  static constexpr int kStages = BITS == 16 ? 3 : 2;  // K/V operand tiles
+  static constexpr int kStages = BITS == 16 ? 3 : 2;   // K operand tiles
+  static constexpr int kVStages = BITS == 16 ? 4 : 2;  // V operand tiles: held until P·V, while K is free after S
   static constexpr int kThreads = BITS == 16 ? 320 : 512;
   static constexpr int kFill = BITS == 16 ? 1 : 6;  // arrivals that fill a K or V tile
 };
 constexpr int kRawMax = 4;
+constexpr int kSBufs = 4;  // S tiles in tensor memory
 
 struct TcArgs {
   TreeArgs t;
@@ -407,9 +410,8 @@ struct TcMap {  // shared memory, bytes from a 1024-byte boundary
   static constexpr int kKBytes = kHalves * kTK * 128;
   static constexpr int kV = kK + TcCfg<BITS>::kStages * kKBytes;
   static constexpr int kVBytes = 2 * kKBytes;
-  static constexpr int kP = kV + TcCfg<BITS>::kStages * kVBytes;
-  static constexpr int kBar = kP + 2 * kTR * 128;
-  static constexpr int kNumBars = 1 + 4 * TcCfg<BITS>::kStages + 4 + 3 + 2 * kRawMax + 12;
+  static constexpr int kBar = kV + TcCfg<BITS>::kVStages * kVBytes;
+  static constexpr int kNumBars = 1 + 2 * TcCfg<BITS>::kStages + 2 * TcCfg<BITS>::kVStages + 3 * kSBufs + 1 + 2 * kRawMax + 12;
   static constexpr int kState = kBar + kNumBars * 8 + 16;  // [128] reference maxima, [2][128] sums of the groups
   static constexpr int kBad = kState + 3 * kTR * 4;        // drafted rows cleared: [2 segments][8 warps] Cleared
   static constexpr int kRaw = (kBad + 2 * 8 * (int)sizeof(Cleared) + 127) / 128 * 128;
@@ -436,6 +438,17 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
   return false;
 }
 
+constexpr int kTestPolls = 1 << 23;  // of two or three tests each: about half a second too
+__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.b32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b);
 template <>
@@ -459,6 +472,14 @@ __device__ __forceinline__ void mma_words(uint32_t d, uint32_t a_lo, uint32_t b_
       "{\n .reg .pred p;\n .reg .b64 da, db;\n mov.b64 da, {%1, %3};\n mov.b64 db, {%2, %3};\n"
       " setp.ne.b32 p, %5, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n}\n" ::"r"(d),
       "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+// The same with A (rows in lanes, two 16-bit values of K a column) in tensor memory.
+__device__ __forceinline__ void mma_tmem_a(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t hi, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 db;\n mov.b64 db, {%2, %3};\n setp.ne.b32 p, %5, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)accumulate)
       : "memory");
 }
 // Any of the two 16-bit values of w is an infinity or NaN.
@@ -565,9 +586,9 @@ template <typename T, int D, int BITS>
 __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const __grid_constant__ TcArgs ta) {
   using Cfg = TcCfg<BITS>;
   using Map = TcMap<D, BITS>;
-  constexpr int NS = Cfg::kStages;
+  constexpr int NS = Cfg::kStages, NV = Cfg::kVStages;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  constexpr uint32_t kColS = 0, kColO = 128, kCols = D == 128 ? 512 : 256;
+  constexpr uint32_t kColS = 0, kColO = kSBufs * kTK, kCols = 512;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const TreeArgs& a = ta.t;
@@ -576,16 +597,17 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
   const uint32_t q_full = bar;
   auto k_full = [&](int s) { return bar + 8u * (1 + s); };
   auto k_empty = [&](int s) { return bar + 8u * (1 + NS + s); };
-  auto v_full = [&](int s) { return bar + 8u * (1 + 2 * NS + s); };
-  auto v_empty = [&](int s) { return bar + 8u * (1 + 3 * NS + s); };
-  auto s_full = [&](int s) { return bar + 8u * (1 + 4 * NS + s); };
-  auto p_full = [&](int s) { return bar + 8u * (3 + 4 * NS + s); };
-  auto o_done = [&](int s) { return bar + 8u * (5 + 4 * NS + s); };  // P·V of tiles of parity s
-  const uint32_t drain = bar + 8u * (7 + 4 * NS);
-  auto raw_full = [&](int s) { return bar + 8u * (8 + 4 * NS + s); };
-  auto raw_empty = [&](int s) { return bar + 8u * (8 + 4 * NS + kRawMax + s); };
-  auto m_next = [&](int g, int q) { return bar + 8u * (8 + 4 * NS + 2 * kRawMax + 4 * g + q); };  // maxima handed on by group g
-  auto l_both = [&](int q) { return bar + 8u * (16 + 4 * NS + 2 * kRawMax + q); };
+  constexpr int kB0 = 1 + 2 * NS, kB1 = kB0 + 2 * NV, kB2 = kB1 + kSBufs, kB3 = kB2 + 2 * kSBufs + 1, kB4 = kB3 + 2 * kRawMax;
+  auto v_full = [&](int s) { return bar + 8u * (kB0 + s); };
+  auto v_empty = [&](int s) { return bar + 8u * (kB0 + NV + s); };
+  auto s_full = [&](int s) { return bar + 8u * (kB1 + s); };
+  auto p_full = [&](int s) { return bar + 8u * (kB2 + s); };  // P, and P·V done, by the S buffer that holds P
+  auto o_done = [&](int s) { return bar + 8u * (kB2 + kSBufs + s); };
+  const uint32_t drain = bar + 8u * (kB2 + 2 * kSBufs);
+  auto raw_full = [&](int s) { return bar + 8u * (kB3 + s); };
+  auto raw_empty = [&](int s) { return bar + 8u * (kB3 + kRawMax + s); };
+  auto m_next = [&](int g, int q) { return bar + 8u * (kB4 + 4 * g + q); };  // maxima handed on by group g
+  auto l_both = [&](int q) { return bar + 8u * (kB4 + 8 + q); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Map::kBar + Map::kNumBars * 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -624,10 +646,10 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
     for (int i = 0; i < Map::kNumBars; ++i) {
       int count = 1;
       if (i == 0) count = 8;                                                                  // q_full
-      if ((i >= 1 && i < 1 + NS) || (i >= 1 + 2 * NS && i < 1 + 3 * NS)) count = Cfg::kFill;  // k_full, v_full
-      if (i >= 3 + 4 * NS && i < 5 + 4 * NS) count = 4;                                       // p_full
-      if (i >= 8 + 4 * NS + kRawMax && i < 8 + 4 * NS + 2 * kRawMax) count = Cfg::kFill;      // raw_empty
-      if (i >= 16 + 4 * NS + 2 * kRawMax) count = 2;                                          // l_both
+      if ((i >= 1 && i < 1 + NS) || (i >= kB0 && i < kB0 + NV)) count = Cfg::kFill;           // k_full, v_full
+      if (i >= kB2 && i < kB2 + kSBufs) count = 4;                                            // p_full
+      if (i >= kB3 + kRawMax && i < kB4) count = Cfg::kFill;                                  // raw_empty
+      if (i >= kB4 + 8) count = 2;                                                            // l_both
       tc::mbar_init(bar + 8u * i, count);
     }
     *abort_flag = 0;
@@ -653,22 +675,21 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
           const int p0 = kt * kTK;
           if (*abort_flag) { ok = false; break; }
           if constexpr (BITS == 16) {
-            const int s = it % NS;
-            const uint32_t par = (it / NS - 1) & 1;
-            if (it >= NS && !bar_wait(k_empty(s), par)) { ok = false; break; }
+            const int s = it % NS, sv = it % NV;
+            if (it >= NS && !bar_wait(k_empty(s), (it / NS - 1) & 1)) { ok = false; break; }
             const uint32_t kb = sb + Map::kK + s * Map::kKBytes;
             tc::mbar_expect_tx(k_full(s), Map::kKBytes);
 #pragma unroll
             for (int h = 0; h < Map::kHalves; ++h)
               tc::tma_load_4d(kb + h * kTK * 128, &ta.tm[0], h * 128, p0, sg.g, sg.b, k_full(s));
             k_iss = it + 1;
-            if (it >= NS && !bar_wait(v_empty(s), par)) { ok = false; break; }
-            const uint32_t vb = sb + Map::kV + s * Map::kVBytes;
-            tc::mbar_expect_tx(v_full(s), Map::kVBytes);
+            if (it >= NV && !bar_wait(v_empty(sv), (it / NV - 1) & 1)) { ok = false; break; }
+            const uint32_t vb = sb + Map::kV + sv * Map::kVBytes;
+            tc::mbar_expect_tx(v_full(sv), Map::kVBytes);
 #pragma unroll
             for (int h = 0; h < 2 * Map::kHalves; ++h)
               tc::tma_load_4d(vb + h * kTK * 128, &ta.tm[1 + h / Map::kHalves], (h % Map::kHalves) * 128, p0, sg.g, sg.b,
-                              v_full(s));
+                              v_full(sv));
             v_iss = it + 1;
           } else {
             const int s = it % ta.raw_stages;
@@ -696,61 +717,66 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
       const int ring = BITS == 16 ? NS : ta.raw_stages;
       for (int j = max(0, k_iss - ring); j < k_iss; ++j)
         if (!bar_wait(BITS == 16 ? k_full(j % ring) : raw_full(j % ring), (j / ring) & 1)) *abort_flag = 1;
-      for (int j = max(0, v_iss - ring); j < v_iss; ++j)
-        if (!bar_wait(v_full(j % ring), (j / ring) & 1)) *abort_flag = 1;
+      for (int j = max(0, v_iss - NV); j < v_iss; ++j)
+        if (!bar_wait(v_full(j % NV), (j / NV) & 1)) *abort_flag = 1;
     }
-  } else if (warp == 1) {  // ---- MMAs: the warp walks the tiles together, one lane issues ----
-    constexpr uint32_t idesc_qk = tc::idesc_f16_f32(kTR, kTK, false, false, kBf16);
-    constexpr uint32_t idesc_pv = tc::idesc_f16_f32(kTR, 2 * D, true, false, kBf16);
-    // Descriptors as words: the upper ones are constants and the lower ones advance by constants, so that the
-    // issuing lane has one addition per product.
-    constexpr uint64_t kd = 1024 >> 4 | 1u << 14 | 2u << 29;  // K-major and MN-major alike: 1024-byte atoms, 128-byte swizzle
-    constexpr uint32_t hi = (uint32_t)kd;
-    const uint32_t q_lo = ((sb + Map::kQ) >> 4) | 1u << 16, k_lo = ((sb + Map::kK) >> 4) | 1u << 16;
-    const uint32_t p_lo = ((sb + Map::kP) >> 4) | 1u << 16, v_lo = ((sb + Map::kV) >> 4) | (kTK * 128 >> 4) << 16;
-    const bool leader = lane == 0;
-    auto issue_qk = [&](int it) -> bool {
-      const int s = it % NS;
-      if (!bar_wait(k_full(s), (it / NS) & 1)) return false;
-      tc::tc_fence_after();
-      if (leader) {
-        const uint32_t kl = k_lo + s * (Map::kKBytes >> 4), d = tmem + kColS + 64 * (it & 1);
+  } else if (warp == 1) {
+    if (lane == 0) {  // ---- MMAs ----
+      constexpr uint32_t idesc_qk = tc::idesc_f16_f32(kTR, kTK, false, false, kBf16);
+      constexpr uint32_t idesc_pv = tc::idesc_f16_f32(kTR, 2 * D, true, false, kBf16);
+      // Descriptors as words: the upper ones are one constant (1024-byte atoms, 128-byte swizzle) and the lower
+      // ones advance by constants, so that a product costs one addition.
+      constexpr uint32_t hi = 1024 >> 4 | 1u << 14 | 2u << 29;
+      const uint32_t q_lo = ((sb + Map::kQ) >> 4) | 1u << 16, k_lo = ((sb + Map::kK) >> 4) | 1u << 16;
+      const uint32_t v_lo = ((sb + Map::kV) >> 4) | (kTK * 128 >> 4) << 16;
+      auto issue_qk = [&](int j) {
+        const int s = j % NS;
+        tc::tc_fence_after();
+        const uint32_t kl = k_lo + s * (Map::kKBytes >> 4), d = tmem + kColS + kTK * (j % kSBufs);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
           mma_words(d, q_lo + (kk >> 2) * (kTR * 128 >> 4) + (kk & 3) * 2, kl + (kk >> 2) * (kTK * 128 >> 4) + (kk & 3) * 2, hi,
                     idesc_qk, kk > 0);
-        tc::mma_commit(s_full(it & 1));
+        tc::mma_commit(s_full(j % kSBufs));
         tc::mma_commit(k_empty(s));
-      }
-      __syncwarp();
-      return true;
-    };
-    int it = 0, seg = 0;
-    bool ok = true;
-    for (; ok && more; more = sched.next(a, sg), ++seg) {
-      ok = bar_wait(q_full, seg & 1) && issue_qk(it);
-      for (int kt = sg.t0; ok && kt < sg.t1; ++kt, ++it) {
-        if (*abort_flag || (kt + 1 < sg.t1 && !issue_qk(it + 1))) { ok = false; break; }
-        const int s = it % NS;
-        if (!bar_wait(p_full(it & 1), (it >> 1) & 1) || !bar_wait(v_full(s), (it / NS) & 1)) { ok = false; break; }
+      };
+      auto issue_pv = [&](int j, bool accumulate) {
         tc::tc_fence_after();
-        if (leader) {
-          const uint32_t pl = p_lo + (it & 1) * (kTR * 128 >> 4), vl = v_lo + s * (Map::kVBytes >> 4);
+        const uint32_t pt = tmem + kColS + kTK * (j % kSBufs), vl = v_lo + (j % NV) * (Map::kVBytes >> 4);
 #pragma unroll
-          for (int kk = 0; kk < kTK / 16; ++kk)
-            mma_words(tmem + kColO, pl + kk * 2, vl + kk * (2048 >> 4), hi, idesc_pv, kt > sg.t0 || kk > 0);
-          tc::mma_commit(o_done(it & 1));
-          tc::mma_commit(v_empty(s));
+        for (int kk = 0; kk < kTK / 16; ++kk)
+          mma_tmem_a(tmem + kColO, pt + kk * 8, vl + kk * (2048 >> 4), hi, idesc_pv, accumulate || kk > 0);
+        tc::mma_commit(o_done(j % kSBufs));
+        tc::mma_commit(v_empty(j % NV));
+      };
+      int it = 0, qn = 0, seg = 0;  // the next P·V, the next S
+      bool ok = true;
+      for (; ok && more; more = sched.next(a, sg), ++seg) {
+        ok = bar_wait(q_full, seg & 1);
+        const int end = it + sg.t1 - sg.t0, begin = it;
+        // S runs up to kSBufs tiles ahead of P·V; its buffer is free once the P·V of kSBufs tiles before has read P there.
+        for (int polls = 0; ok && it < end;) {
+          const bool s_ahead = qn < end && qn < it + kSBufs &&
+                               (qn < kSBufs || bar_test(o_done(qn % kSBufs), (qn / kSBufs - 1) & 1));
+          if (s_ahead && (qn <= it + 1 || !bar_test(p_full(it % kSBufs), (it / kSBufs) & 1)) &&
+              bar_test(k_full(qn % NS), (qn / NS) & 1)) {
+            issue_qk(qn++);
+            polls = 0;
+          } else if (qn > it && bar_test(p_full(it % kSBufs), (it / kSBufs) & 1) && bar_test(v_full(it % NV), (it / NV) & 1)) {
+            issue_pv(it, it > begin);
+            ++it;
+            polls = 0;
+          } else if (++polls > kTestPolls || *abort_flag) {
+            ok = false;
+          }
         }
-        __syncwarp();
       }
-      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) *abort_flag = 1;
+      // every MMA this thread issued completes before tensor memory can be freed
+      tc::mma_commit(drain);
+      if (!bar_wait(drain, 0)) *abort_flag = 1;
     }
-    if (!ok) *abort_flag = 1;
-    // every MMA this warp issued completes before tensor memory can be freed
-    if (leader) tc::mma_commit(drain);
     __syncwarp();
-    if (!bar_wait(drain, 0)) *abort_flag = 1;
   } else if (warp < 10) {  // ---- softmax: one thread per query row, two groups ----
     const uint32_t trow = tmem + ((uint32_t)(q * 32) << 16);
     const float mult = fabsf(a.scale_log2);
@@ -797,10 +823,9 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
         const int p0 = kt * kTK;
         const bool tail = p0 + kTK > ctx;  // drafted rows or the cache's end in this tile
         const uint64_t vis = tail && live ? visible(a, mrow, sg.b, t, ctx, p0) : 0;
-        if (!(alive = wait(s_full(grp), it >> 1))) continue;
+        if (!(alive = wait(s_full(it % kSBufs), it / kSBufs))) continue;
         tc::tc_fence_after();
-        const uint32_t ts = trow + kColS + 64 * grp;
-        uint8_t* prow = smem + Map::kP + grp * kTR * 128 + r * 128;
+        const uint32_t ts = trow + kColS + kTK * (it % kSBufs);
         bool need = false;
         float factor = 1.f, mb = 0.f, mul = mult;
         constexpr bool kKeep = BITS == 16;  // registers for all 64 columns; else they are read twice
@@ -851,8 +876,8 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
           mb = m_new == -INFINITY ? 0.f : m_new;
         }
         if (tail) {  // clear the V rows a zero weight may not meet
-          const int st = it % NS;
-          if (!(alive = wait(v_full(st), it / NS))) continue;
+          const int st = it % NV;
+          if (!(alive = wait(v_full(st), it / NV))) continue;
           const int vr = q * 16 + (lane >> 1), pos = p0 + vr;
           bool clear = pos >= sg.n;
           uint8_t* vrow = smem + Map::kV + st * Map::kVBytes + (lane & 1) * Map::kHalves * kTK * 128 + vr * 128;
@@ -886,31 +911,27 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
             if (drafted && (lane & 1) == 0) atomicOr(&mine->bits[(pos - ctx) >> 5], 1u << ((pos - ctx) & 31));
           }
         }
-        // the P buffer is free once this group's last P·V has completed
-        if (it >= 2 && !(alive = wait(o_done(grp), (it - 2) >> 1))) continue;
-        if (work) {
+        if (work) {  // P in the type (one rounding of each weight), over the first half of its S
           float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             float(&x)[32] = sv[kKeep ? h : 0];
             if constexpr (!kKeep) load_s(h, x);
+            uint32_t pk[16];
 #pragma unroll
-            for (int c8 = 0; c8 < 4; ++c8) {
-              uint32_t pk[4];
-#pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                const float e0 = ex2(fmaf(x[8 * c8 + 2 * c], mul, -mb)), e1 = ex2(fmaf(x[8 * c8 + 2 * c + 1], mul, -mb));
-                ps[c] += e0 + e1;
-                pk[c] = pack2<T>(e0, e1);  // P in the type: one rounding of each weight
-              }
-              *reinterpret_cast<uint4*>(prow + (((4 * h + c8) ^ (r & 7)) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+            for (int c = 0; c < 16; ++c) {
+              const float e0 = ex2(fmaf(x[2 * c], mul, -mb)), e1 = ex2(fmaf(x[2 * c + 1], mul, -mb));
+              ps[c & 3] += e0 + e1;
+              pk[c] = pack2<T>(e0, e1);
             }
+            tc::tmem_st16(ts + 16 * h, pk);
           }
+          tc::tmem_st_wait();
           l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
         }
         // O takes a raised maximum once the last tile's P·V has completed
         if (kt > sg.t0 && __any_sync(0xffffffffu, need)) {
-          if (!(alive = wait(o_done(grp ^ 1), (it - 1) >> 1))) continue;
+          if (!(alive = wait(o_done((it - 1) % kSBufs), (it - 1) / kSBufs))) continue;
           tc::tc_fence_after();
 #pragma unroll 1
           for (int cb = 0; cb < 2 * D / 32; ++cb) {
@@ -923,22 +944,22 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
           }
           tc::tmem_st_wait();
         }
-        tc::fence_proxy_async_smem();
+        if (tail) tc::fence_proxy_async_smem();  // the cleared rows
         tc::tc_fence_before();
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(p_full(grp));
+        if (lane == 0) tc::mbar_arrive(p_full(it % kSBufs));
       }
       Segment nx;
       more = sched.next(a, nx);
       if (BITS == 4 && more) fetch_q(nx);
       const int e = it - 1;  // the segment's last tile
-      if (alive) alive = wait(s_full(e & 1), e >> 1);
+      if (alive) alive = wait(s_full(e % kSBufs), e / kSBufs);
       // its S is complete: Q is free, and the next segment's first product can start
       if (more && alive) {
         if (BITS != 4) fetch_q(nx);
         store_q();
       }
-      if (alive) alive = wait(o_done(e & 1), e >> 1);
+      if (alive) alive = wait(o_done(e % kSBufs), e / kSBufs);
       tc::tc_fence_after();
       if (work) {
         float m_ref = -INFINITY;
@@ -1001,7 +1022,7 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
         const int rs = it % ta.raw_stages, s = it % NS;
         const uint32_t par = (it / NS - 1) & 1;
         const bool ok = bar_wait(raw_full(rs), (it / ta.raw_stages) & 1) &&
-                        (it < NS || (bar_wait(k_empty(s), par) && bar_wait(v_empty(s), par)));
+                        (it < NS || (bar_wait(k_empty(s), par) && bar_wait(v_empty(s), par)));  // NV is NS here
         if (__any_sync(0xffffffffu, !ok || *abort_flag)) { alive = false; break; }
         const uint8_t* raw = smem + Map::kRaw + rs * (3 * kTK * ta.code_bytes + 6 * kTK * ta.group_bytes);
         for (int u = tid; u < 3 * kUnits; u += Cfg::kThreads - 320) {  // 3·kUnits is a multiple of the threads
