@@ -599,9 +599,11 @@ MOTIF_API int motif_speculative_accept(const void* p_logits, const void* q_logit
  * [0, vocab) is never accepted (padding); NaN logits count as -inf; a target
  * row without a finite logit accepts nothing and yields token 0.
  * accepted (B): drafted tokens accepted; path (B, rows): 0, the accepted rows,
- * then -1. Strides in elements. The reference's rule for one chain with its
+ * then -1. Strides in elements (the logits on their type's boundary).
+ * workspace: any contents; calls that may overlap need one each. The reference's rule for one chain with its
  * own random numbers is motif_speculative_accept's. */
-MOTIF_API size_t motif_speculative_verify_workspace_bytes(int64_t batch, int64_t rows, int64_t draft_rows);
+MOTIF_API size_t motif_speculative_verify_workspace_bytes(int64_t batch, int64_t rows, int64_t draft_rows,
+                                                         int64_t vocab);
 MOTIF_API int motif_speculative_verify(int dtype, const void* p_logits, int64_t p_batch_stride, int64_t p_row_stride,
                                        const void* q_logits, int64_t q_batch_stride, int64_t q_row_stride,
                                        int64_t draft_rows, const int32_t* tokens, const int32_t* parents,

@@ -14,6 +14,20 @@
 // The drawn token is the first x whose running sum of w exceeds u_0 times the whole. A vocabulary has
 // as many borders between tokens as entries: with sums or exponentials in 32 bits (2^-24 relative) some
 // 1% of the draws over 2·10^5 entries would fall to the other side of one, so they are in 64 bits.
+//
+// Two launches:
+//   verify_stats_kernel reads every row once at memory speed: per 8192-entry chunk the maximum and Σ exp
+//     against it in 32 bits (the walk repeats a test that this cannot decide with sums in 64 bits), or at τ = 0 the largest logit and its first index;
+//   verify_walk_kernel walks the tree, one thread-block cluster a sequence. All CTAs of a cluster take the
+//     same decisions from the chunks' values; where a child is rejected they sum their parts of the row's
+//     S_j in 64 bits and exchange the sums through distributed shared memory (each part added in the same
+//     order by everyone, so the CTAs stay in step without another word). The draw finds the CTA, then the
+//     warp's range, then the entry.
+// The walk is bound by latency and by the 64-bit pipes: a pass over a row pair of 219520 entries is 439 k
+// exponentials of ~20 64-bit operations on the cluster's SMs.
+#include <cooperative_groups.h>
+
+#include <atomic>
 #include <cmath>
 
 #include "common.cuh"
@@ -21,7 +35,13 @@
 namespace motif {
 namespace {
 
-constexpr int kVThreads = 1024;
+
+constexpr int kChunk = 8192, kStatThreads = 256;
+constexpr int kWalkThreads = 512, kWalkWarps = kWalkThreads / 32;
+constexpr int kMaxRows = 1024, kMaxCluster = 16;
+// The 32-bit row sums are within 2^-17 (exponent's rounding at |x| ≤ 60: 2^-18; 64 additions: 2^-18). A test closer
+// to its border than this is repeated with sums in 64 bits, both rows added in the same order.
+constexpr double kMargin = 1.0 / 32768;
 
 struct VerifyArgs {
   const void *p, *q;
@@ -30,7 +50,9 @@ struct VerifyArgs {
   int64_t parents_b;
   const float* u;
   int32_t *accepted, *path, *next;
-  int T, R, V;
+  float2* stats;             // [B][T + R][chunks]: maximum, Σ exp
+  unsigned long long* tops;  // τ = 0: [B][T][chunks] keys
+  int T, R, V, chunks;
   double inv_t;  // 0: greedy
 };
 
@@ -44,173 +66,405 @@ __device__ __forceinline__ double weight(float l, float m, double inv_t) {
   return m == -INFINITY ? 0.0 : l == m ? 1.0 : exp(((double)l - (double)m) * inv_t);
 }
 
-__device__ double block_sum_f64(double v, double* sm) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if (lane == 0) sm[warp] = v;
-  __syncthreads();
-  v = sm[lane];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
-// Largest logit of a row and its first index, as one order-preserving key.
-template <typename T>
-__device__ unsigned long long block_top(const T* l, int V, unsigned long long* sm) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  unsigned long long best = 0;
-  for (int i = threadIdx.x; i < V; i += kVThreads) {
-    uint32_t b = __float_as_uint(logit(l, i) + 0.f);  // −0 ties with 0
-    b = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-    const unsigned long long k = ((unsigned long long)b << 32) | (0xFFFFFFFFu - (uint32_t)i);
-    best = k > best ? k : best;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long w = __shfl_xor_sync(0xffffffffu, best, o);
-    best = w > best ? w : best;
-  }
-  __syncthreads();
-  if (lane == 0) sm[warp] = best;
-  __syncthreads();
-  best = sm[lane];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long w = __shfl_xor_sync(0xffffffffu, best, o);
-    best = w > best ? w : best;
-  }
-  return best;
+// Order-preserving key of (value, index): the larger value, then the smaller index.
+__device__ __forceinline__ unsigned long long top_key(float v, int i) {
+  uint32_t b = __float_as_uint(v + 0.f);  // −0 ties with 0
+  b = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  return ((unsigned long long)b << 32) | (0xFFFFFFFFu - (uint32_t)i);
 }
 __device__ __forceinline__ float key_value(unsigned long long k) {
   const uint32_t b = (uint32_t)(k >> 32);
   return __uint_as_float((b & 0x80000000u) ? (b & 0x7FFFFFFFu) : ~b);
 }
 __device__ __forceinline__ int key_index(unsigned long long k) { return (int)(0xFFFFFFFFu - (uint32_t)k); }
+__device__ __forceinline__ unsigned long long warp_max_u64(unsigned long long v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const unsigned long long w = __shfl_xor_sync(0xffffffffu, v, o);
+    v = w > v ? w : v;
+  }
+  return v;
+}
+
+// One chunk of one row: [lo, hi), lo on a 16-byte boundary of the row but for the first chunk, whose few entries
+// before the boundary are its `head`.
+template <typename T>
+__global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(VerifyArgs a) {
+  constexpr int kVec = 16 / (int)sizeof(T), kLoads = kChunk / kVec / kStatThreads;
+  __shared__ float sf[8];
+  __shared__ unsigned long long sk[8];
+  const int row = blockIdx.y, c = blockIdx.x, b = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_trigger();
+  const T* l = row < a.T ? static_cast<const T*>(a.p) + b * a.pb + row * a.pr
+                         : static_cast<const T*>(a.q) + b * a.qb + (row - a.T) * a.qr;
+  const int shift = min((int)((16 - reinterpret_cast<uintptr_t>(l) % 16) % 16 / sizeof(T)), a.V);
+  const int lo = min(c * kChunk + shift, a.V), hi = c + 1 == a.chunks ? a.V : min(lo + kChunk, a.V);
+  const int n_vec = (hi - lo) / kVec;
+  uint4 raw[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int v = tid + i * kStatThreads;
+    if (v < n_vec) raw[i] = reinterpret_cast<const uint4*>(l + lo)[v];
+  }
+  // the entries outside whole vectors: before the first chunk's boundary, and behind the last vector
+  const int tail0 = lo + n_vec * kVec;
+  int edge = -1;
+  if (c == 0 && tid < shift) edge = tid;
+  if (tid >= 32 && tail0 + tid - 32 < hi) edge = tail0 + tid - 32;
+  const float ev = edge >= 0 ? logit(l, edge) : -INFINITY;
+  float m = ev;
+  unsigned long long top = edge >= 0 ? top_key(ev, edge) : 0;
+  const bool greedy = a.inv_t == 0.0;
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int v = tid + i * kStatThreads;
+    if (v >= n_vec) continue;
+    const T* e = reinterpret_cast<const T*>(&raw[i]);
+#pragma unroll
+    for (int x = 0; x < kVec; ++x) {
+      const float f = logit(e, x);
+      m = fmaxf(m, f);
+      if (greedy) {
+        const unsigned long long k = top_key(f, lo + v * kVec + x);
+        top = k > top ? k : top;
+      }
+    }
+  }
+  if (greedy) {
+    top = warp_max_u64(top);
+    if (lane == 0) sk[warp] = top;
+    __syncthreads();
+    if (tid == 0) {
+#pragma unroll
+      for (int w = 1; w < 8; ++w) top = sk[w] > top ? sk[w] : top;
+      a.tops[((int64_t)b * a.T + row) * a.chunks + c] = top;
+    }
+    return;
+  }
+  m = warp_max(m);
+  if (lane == 0) sf[warp] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) m = fmaxf(m, sf[w]);
+  const float k = (float)a.inv_t * 1.4426950408889634f;
+  auto term = [&](float f) { return f == m ? 1.f : exp2f((f - m) * k); };  // m may be infinite
+  float z = edge >= 0 && m > -INFINITY ? term(ev) : 0.f;
+  if (m > -INFINITY) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int v = tid + i * kStatThreads;
+      if (v >= n_vec) continue;
+      const T* e = reinterpret_cast<const T*>(&raw[i]);
+#pragma unroll
+      for (int x = 0; x < kVec; ++x) z += term(logit(e, x));
+    }
+  }
+  z = warp_sum(z);
+  __syncthreads();
+  if (lane == 0) sf[warp] = z;
+  __syncthreads();
+  if (tid == 0) {
+    z = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) z += sf[w];
+    a.stats[((int64_t)b * (a.T + a.R) + row) * a.chunks + c] = make_float2(m, z);
+  }
+}
 
 struct Law {
   float m;
   double inv_z;
 };
-template <typename T>
-__device__ Law row_law(const T* l, int V, double inv_t, double* smd, unsigned long long* smk) {
-  Law w;
-  w.m = key_value(block_top(l, V, smk));
-  double z = 0.0;
-  for (int i = threadIdx.x; i < V; i += kVThreads) z += weight(logit(l, i), w.m, inv_t);
-  z = block_sum_f64(z, smd);
-  w.inv_z = z > 0.0 ? 1.0 / z : 0.0;
-  return w;
+
+__device__ __forceinline__ double warp_sum_f64(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
 
+// One cluster per sequence; CTA `rank` owns the vocabulary range [rank·V/C, (rank+1)·V/C), a warp a sixteenth of it.
 template <typename T>
-__global__ void __launch_bounds__(kVThreads) verify_kernel(VerifyArgs a) {
-  __shared__ double smd[32], part[kVThreads];
-  __shared__ unsigned long long smk[32];
-  __shared__ int s_token;
-  const int b = blockIdx.x, tid = threadIdx.x;
+__global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyArgs a) {
+  namespace cg = cooperative_groups;
+  extern __shared__ __align__(16) uint8_t dyn[];
+  __shared__ double ws[kWalkWarps], sums[2][kMaxCluster][2];
+  __shared__ double scan[kWalkWarps];
+  __shared__ int found;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int b = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // per tree row: parent, token, uniform; logits of its token in its parent's rows; laws of its own rows
+  int* par = reinterpret_cast<int*>(dyn);
+  int* tok = par + a.T;
+  float* u = reinterpret_cast<float*>(tok + a.T);
+  float* px = u + a.T;
+  float* qx = px + a.T;
+  float* pm = qx + a.T;
+  float* qm = pm + a.T;
+  double* pz = reinterpret_cast<double*>(dyn + ((7 * a.T * 4 + 15) & ~15));  // 1 / Σ
+  double* qz = pz + a.T;
   const T* P = static_cast<const T*>(a.p) + b * a.pb;
   const T* Q = static_cast<const T*>(a.q) + b * a.qb;
-  const int32_t* tok = a.tokens + (int64_t)b * a.T;
-  const int32_t* par = a.parents + b * a.parents_b;
-  const float* u = a.u + (int64_t)b * a.T;
-  int32_t* path = a.path + (int64_t)b * a.T;
   const bool greedy = a.inv_t == 0.0;
+  for (int i = tid; i < a.T; i += kWalkThreads) {
+    const int pa = i ? a.parents[b * a.parents_b + i] : -1, x = a.tokens[(int64_t)b * a.T + i];
+    par[i] = pa;
+    tok[i] = x;
+    if (greedy) continue;
+    u[i] = a.u[(int64_t)b * a.T + i];
+    const bool test = pa >= 0 && pa < i && x >= 0 && x < a.V;
+    px[i] = test ? logit(P + pa * a.pr, x) : -INFINITY;
+    qx[i] = test && pa < a.R ? logit(Q + pa * a.qr, x) : -INFINITY;
+  }
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  // the rows' laws (τ = 0: their largest entries) from the chunks: eight lanes a row
+  for (int r0 = tid / 8; r0 < a.T + (greedy ? 0 : a.R); r0 += kWalkThreads / 8) {
+    const unsigned mask = 0xFFu << (lane & 24);
+    if (greedy) {
+      unsigned long long k = 0;
+      for (int c = lane & 7; c < a.chunks; c += 8) {
+        const unsigned long long v = a.tops[((int64_t)b * a.T + r0) * a.chunks + c];
+        k = v > k ? v : k;
+      }
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) {
+        const unsigned long long v = __shfl_xor_sync(mask, k, o);
+        k = v > k ? v : k;
+      }
+      if ((lane & 7) == 0) reinterpret_cast<unsigned long long*>(pz)[r0] = k;
+      continue;
+    }
+    const float2* st = a.stats + ((int64_t)b * (a.T + a.R) + r0) * a.chunks;
+    float m = -INFINITY;
+    for (int c = lane & 7; c < a.chunks; c += 8) m = fmaxf(m, st[c].x);
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(mask, m, o));
+    double z = 0.0;
+    for (int c = lane & 7; c < a.chunks; c += 8) {
+      const float2 s = st[c];
+      z += s.x == m ? (double)s.y : s.x == -INFINITY ? 0.0 : (double)s.y * exp(((double)s.x - (double)m) * a.inv_t);
+    }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) z += __shfl_xor_sync(mask, z, o);
+    if ((lane & 7) == 0) {
+      (r0 < a.T ? pm : qm)[r0 < a.T ? r0 : r0 - a.T] = m;
+      (r0 < a.T ? pz : qz)[r0 < a.T ? r0 : r0 - a.T] = m > -INFINITY && z > 0.0 ? 1.0 / z : 0.0;
+    }
+  }
+  __syncthreads();
+
+  if (greedy) {
+    const unsigned long long* top = reinterpret_cast<const unsigned long long*>(pz);
+    if (tid == 0) {
+      int cur = 0, kept = 1;
+      auto best = [&](int r) { return key_value(top[r]) > -INFINITY ? key_index(top[r]) : -1; };
+      int want = best(0);
+      int32_t* path = a.path + (int64_t)b * a.T;
+      path[0] = 0;
+      for (int i = 1; i < a.T; ++i)
+        if (par[i] == cur && want >= 0 && tok[i] == want) {
+          cur = i;
+          path[kept++] = i;
+          want = best(i);
+        }
+      for (int i = kept; i < a.T; ++i) path[i] = -1;
+      a.accepted[b] = kept - 1;
+      a.next[b] = max(want, 0);
+    }
+    return;
+  }
+
+  const int v0 = (int)((int64_t)rank * a.V / C), v1 = (int)((int64_t)(rank + 1) * a.V / C);
+  auto range = [&](int w) { return v0 + (int)((int64_t)w * (v1 - v0) / kWalkWarps); };
+  const int w0 = range(warp), w1 = range(warp + 1);
+  int phase = 0;
+  // Sums of two values over the cluster, the same on every CTA; my warps' sums of the first stay in ws.
+  auto total = [&](double x, double y, double& sx, double& sy) {
+    x = warp_sum_f64(x), y = warp_sum_f64(y);
+    __syncthreads();
+    if (lane == 0) ws[warp] = x, scan[warp] = y;
+    __syncthreads();
+    if (tid < C) {  // my CTA's sums into every CTA's slots
+      double cx = 0.0, cy = 0.0;
+      for (int w = 0; w < kWalkWarps; ++w) cx += ws[w], cy += scan[w];
+      double* dst = cluster.map_shared_rank(&sums[phase][rank][0], tid);
+      dst[0] = cx, dst[1] = cy;
+    }
+    cluster.sync();
+    sx = sy = 0.0;
+    for (int c = 0; c < C; ++c) sx += sums[phase][c][0], sy += sums[phase][c][1];
+    phase ^= 1;  // the other slots' readers are behind the next sync
+  };
   int cur = 0, kept = 1;
   double coef = 0.0, S = 1.0;
-  bool have_q = false;
-  Law lp{}, lq{};
-  unsigned long long top = 0;
-  auto enter = [&](int r) {
-    if (greedy) top = block_top(P + r * a.pr, a.V, smk);
-    else lp = row_law(P + r * a.pr, a.V, a.inv_t, smd, smk);
+  Law lp{pm[0], pz[0]}, lq{};
+  bool exact = false;  // the laws' sums in 64 bits
+  int32_t* path = a.path + (int64_t)b * a.T;
+  if (rank == 0 && tid == 0) path[0] = 0;
+  auto wp = [&](const T* p, int e) { return weight(logit(p, e), lp.m, a.inv_t) * lp.inv_z; };
+  auto wq = [&](const T* q, int e) { return weight(logit(q, e), lq.m, a.inv_t) * lq.inv_z; };
+  auto make_exact = [&](const T* p, const T* q, bool with_q) {
+    double x = 0.0, y = 0.0, sx, sy;
+    for (int e = w0 + lane; e < w1; e += 32) {
+      x += weight(logit(p, e), lp.m, a.inv_t);
+      if (with_q) y += weight(logit(q, e), lq.m, a.inv_t);
+    }
+    total(x, y, sx, sy);
+    lp.inv_z = sx > 0.0 ? 1.0 / sx : 0.0;
+    if (with_q) lq.inv_z = sy > 0.0 ? 1.0 / sy : 0.0;
+    exact = true;
   };
-  enter(0);
-  for (int i = tid; i < a.T; i += kVThreads) path[i] = i == 0 ? 0 : -1;
-  __syncthreads();
   for (int i = 1; i < a.T; ++i) {
     if (par[i] != cur) continue;
     const int x = tok[i];
-    if (x < 0 || x >= a.V) continue;  // a padding row
-    bool ok;
-    if (greedy) {
-      ok = key_value(top) > -INFINITY && x == key_index(top);
-    } else {
-      if (cur >= a.R) continue;  // no draft row: nothing can be tested
-      const T* p = P + cur * a.pr;
-      const T* q = Q + cur * a.qr;
-      if (!have_q) lq = row_law(q, a.V, a.inv_t, smd, smk), have_q = true;
-      const double px = weight(logit(p, x), lp.m, a.inv_t) * lp.inv_z;
-      const double qx = weight(logit(q, x), lq.m, a.inv_t) * lq.inv_z;
-      ok = (double)u[i] * qx * S < px - coef * qx;
-      if (!ok) {
-        coef += S;
-        double s = 0.0;
-        for (int e = tid; e < a.V; e += kVThreads)
-          s += fmax(0.0, weight(logit(p, e), lp.m, a.inv_t) * lp.inv_z - coef * (weight(logit(q, e), lq.m, a.inv_t) * lq.inv_z));
-        S = block_sum_f64(s, smd);
-      }
-    }
-    if (ok) {
-      cur = i;
-      if (tid == 0) path[kept] = i;
-      ++kept;
-      coef = 0.0, S = 1.0, have_q = false;
-      enter(i);
-    }
-  }
-  if (greedy) {
-    if (tid == 0) s_token = key_value(top) > -INFINITY ? key_index(top) : 0;
-  } else {
-    // contiguous chunks: their sums, then the chunk that holds the border, then the entry
-    if (!(S > 0.0)) coef = 0.0;  // an empty residual: the target's own law
+    if (x < 0 || x >= a.V || cur >= a.R) continue;  // a padding row; a row without a draft row
     const T* p = P + cur * a.pr;
-    const T* q = Q + (cur < a.R ? cur : 0) * a.qr;
-    const int per = (a.V + kVThreads - 1) / kVThreads, e0 = min(tid * per, a.V), e1 = min(e0 + per, a.V);
-    auto w = [&](int e) {
-      const double pe = weight(logit(p, e), lp.m, a.inv_t) * lp.inv_z;
-      return coef == 0.0 ? pe : fmax(0.0, pe - coef * (weight(logit(q, e), lq.m, a.inv_t) * lq.inv_z));
-    };
-    double s = 0.0;
-    for (int e = e0; e < e1; ++e) s += w(e);
-    part[tid] = s;
+    const T* q = Q + cur * a.qr;
+    if (!exact) lq = Law{qm[cur], qz[cur]};
+    double pe = weight(px[i], lp.m, a.inv_t) * lp.inv_z, qe = weight(qx[i], lq.m, a.inv_t) * lq.inv_z;
+    if (!exact && fabs((double)u[i] * qe * S - (pe - coef * qe)) <= kMargin * (pe + qe)) {
+      make_exact(p, q, true);
+      pe = weight(px[i], lp.m, a.inv_t) * lp.inv_z, qe = weight(qx[i], lq.m, a.inv_t) * lq.inv_z;
+    }
+    if ((double)u[i] * qe * S < pe - coef * qe) {
+      if (rank == 0 && tid == 0) path[kept] = i;
+      ++kept;
+      cur = i;
+      coef = 0.0, S = 1.0, exact = false;
+      lp = Law{pm[i], pz[i]};
+      continue;
+    }
+    if (!exact) make_exact(p, q, true);
+    coef += S;
+    double s = 0.0, unused;
+    for (int e = w0 + lane; e < w1; e += 32) s += fmax(0.0, wp(p, e) - coef * wq(q, e));
+    total(s, 0.0, S, unused);
+  }
+  // the draw, from (p − coef·q)⁺ or (no rejection, or an empty residual) from p
+  const T* p = P + cur * a.pr;
+  const T* q = Q + (cur < a.R ? cur : 0) * a.qr;
+  double W = S;
+  if (coef == 0.0 || !(S > 0.0)) {
+    coef = 0.0;
+    double s = 0.0, unused;
+    for (int e = w0 + lane; e < w1; e += 32) s += weight(logit(p, e), lp.m, a.inv_t);
+    lp.inv_z = 1.0;
+    total(s, 0.0, W, unused);
+  }
+  auto w = [&](int e) { return coef == 0.0 ? weight(logit(p, e), lp.m, a.inv_t) : fmax(0.0, wp(p, e) - coef * wq(q, e)); };
+  // the CTA, then the warp's range that holds the border; the last one with any weight if rounding leaves none beyond it
+  const double target = (double)u[0] * W;
+  double before = 0.0;
+  int cta = -1, sub = -1;
+  for (int c = 0; c < C; ++c) {
+    const double x = sums[phase ^ 1][c][0];
+    if (!(x > 0.0)) continue;
+    cta = c;
+    if (before + x > target) break;
+    before += x;
+  }
+  if (cta < 0) {  // a row without a finite logit
+    if (rank == 0 && tid == 0) a.next[b] = 0;
+  } else if (cta == rank) {
+    for (int k = 0; k < kWalkWarps; ++k) {
+      const double x = ws[k];
+      if (!(x > 0.0)) continue;
+      sub = k;
+      if (before + x > target) break;
+      before += x;
+    }
+    const int e0 = range(sub), e1 = range(sub + 1), per = (e1 - e0 + kWalkThreads - 1) / kWalkThreads;
+    const int mine0 = min(e0 + tid * per, e1), mine1 = min(mine0 + per, e1);
+    double mine = 0.0;
+    int last = -1;
+    for (int e = mine0; e < mine1; ++e) {
+      const double x = w(e);
+      mine += x;
+      if (x > 0.0) last = e;
+    }
+    double run = mine;  // inclusive scan over the CTA
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double x = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += x;
+    }
+    if (tid == 0) found = 0x7fffffff;
+    if (lane == 31) scan[warp] = run;
     __syncthreads();
-    if (tid == 0) {
-      double total = 0.0;
-      for (int i = 0; i < kVThreads; ++i) total += part[i];
-      const double target = (double)u[0] * total;
-      double run = 0.0;
-      int token = 0;
-      bool found = false;
-      for (int i = 0; i < kVThreads && !found; ++i) {
-        if (part[i] > 0.0 && (run + part[i] > target)) {
-          double r = run;
-          for (int e = i * per; e < min((i + 1) * per, a.V) && !found; ++e) {
-            const double we = w(e);
-            if (we > 0.0) token = e;
-            r += we;
-            found = we > 0.0 && r > target;
-          }
-        } else if (part[i] > 0.0) {  // kept in case rounding leaves none beyond the target: the last one
-          token = -1 - i;
-        }
-        run += part[i];
+    for (int k = 0; k < warp; ++k) before += scan[k];
+    run += before;
+    if (mine > 0.0 && run > target) {
+      double r = run - mine;
+      int at = last;
+      for (int e = mine0; e < mine1; ++e) {
+        const double x = w(e);
+        r += x;
+        if (x > 0.0 && r > target) { at = e; break; }
       }
-      if (token < 0) {
-        const int i = -1 - token;
-        for (int e = i * per; e < min((i + 1) * per, a.V); ++e)
-          if (w(e) > 0.0) token = e;
-      }
-      s_token = token < 0 ? 0 : token;
+      atomicMin(&found, at);
+    }
+    __syncthreads();
+    const bool none = found == 0x7fffffff;
+    __syncthreads();
+    if (none) {  // u_0 at or beyond the end
+      if (tid == 0) found = -1;
+      __syncthreads();
+      if (last >= 0) atomicMax(&found, last);
+      __syncthreads();
+    }
+    if (tid == 0) a.next[b] = max(found, 0);
+  }
+  if (rank == 0) {
+    if (tid == 0) a.accepted[b] = kept - 1;
+    for (int i = kept + tid; i < a.T; i += kWalkThreads) path[i] = -1;
+  }
+  cluster.sync();  // no CTA ends while another may still write into its shared memory
+}
+
+int chunks_of(int64_t V) { return (int)ceil_div(V, kChunk); }
+
+template <typename T>
+int launch_verify(const VerifyArgs& a, int64_t batch, cudaStream_t st) {
+  const bool greedy = a.inv_t == 0.0;
+  verify_stats_kernel<T><<<dim3((unsigned)a.chunks, (unsigned)(a.T + (greedy ? 0 : a.R)), (unsigned)batch), kStatThreads, 0, st>>>(a);
+  const int rc = check_launch("speculative_verify");
+  if (rc) return rc;
+  // CTAs of a cluster: all SMs together serve the batch, and a CTA has 2048 entries or more
+  int C = 1;
+  while (!greedy && C < kMaxCluster && 2 * C * batch <= 128 && a.V / (2 * C) >= 2048) C *= 2;
+  auto kern = verify_walk_kernel<T>;
+  const size_t smem = ((7 * (size_t)a.T * 4 + 15) & ~(size_t)15) + 2 * (size_t)a.T * 8;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return fail(MOTIF_ERR_CUDA, "speculative_verify: cluster attribute: %s", cudaGetErrorString(e));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(batch * C));
+  cfg.blockDim = dim3(kWalkThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2]{};
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)C;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  if (C > 8) {  // clusters of 16 need a part of the GPU with 16 SMs: asked once
+    static std::atomic<int> fits{-1};
+    if (fits < 0) {
+      int n = 0;
+      fits = cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess && n > 0;
+      (void)cudaGetLastError();
+    }
+    if (!fits) {
+      C = 8;
+      cfg.gridDim = dim3((unsigned)(batch * C));
+      at[1].val.clusterDim.x = 8;
     }
   }
-  __syncthreads();
-  if (tid == 0) {
-    a.accepted[b] = kept - 1;
-    a.next[b] = s_token;
-  }
+  e = cudaLaunchKernelEx(&cfg, kern, a);
+  if (e != cudaSuccess) return fail(MOTIF_ERR_CUDA, "speculative_verify: %s", cudaGetErrorString(e));
+  return MOTIF_OK;
 }
 
 }  // namespace
@@ -220,9 +474,9 @@ using namespace motif;
 
 extern "C" {
 
-size_t motif_speculative_verify_workspace_bytes(int64_t batch, int64_t rows, int64_t draft_rows) {
-  (void)batch, (void)rows, (void)draft_rows;
-  return 16;
+size_t motif_speculative_verify_workspace_bytes(int64_t batch, int64_t rows, int64_t draft_rows, int64_t vocab) {
+  if (batch < 1 || rows < 1 || draft_rows < 0 || vocab < 1) return 0;
+  return 8 * (size_t)batch * (size_t)(rows + draft_rows) * (size_t)chunks_of(vocab);
 }
 
 int motif_speculative_verify(int dtype, const void* p_logits, int64_t p_batch_stride, int64_t p_row_stride,
@@ -237,7 +491,7 @@ int motif_speculative_verify(int dtype, const void* p_logits, int64_t p_batch_st
                 "speculative_verify: temperature %f", temperature);
   MOTIF_REQUIRE(temperature == 0.0 || (q_logits && uniforms), MOTIF_ERR_NULL,
                 "speculative_verify: q_logits and uniforms are needed at temperature %f", temperature);
-  MOTIF_REQUIRE(batch >= 1 && batch < 65536 && rows >= 1 && rows <= 1024 && vocab >= 1 && vocab < (1ll << 31),
+  MOTIF_REQUIRE(batch >= 1 && batch < 65536 && rows >= 1 && rows <= kMaxRows && vocab >= 1 && vocab < (1ll << 31),
                 MOTIF_ERR_BAD_SHAPE, "speculative_verify: batch=%lld rows=%lld (1..1024) vocab=%lld", (long long)batch,
                 (long long)rows, (long long)vocab);
   MOTIF_REQUIRE(temperature == 0.0 || (draft_rows >= 1 && draft_rows <= rows), MOTIF_ERR_BAD_SHAPE,
@@ -246,7 +500,7 @@ int motif_speculative_verify(int dtype, const void* p_logits, int64_t p_batch_st
                 MOTIF_ERR_BAD_SHAPE, "speculative_verify: negative stride");
   MOTIF_REQUIRE(parents_batch_stride == 0 || parents_batch_stride == rows, MOTIF_ERR_BAD_SHAPE,
                 "speculative_verify: parents batch stride %lld", (long long)parents_batch_stride);
-  const size_t need = motif_speculative_verify_workspace_bytes(batch, rows, draft_rows);
+  const size_t need = motif_speculative_verify_workspace_bytes(batch, rows, temperature > 0.0 ? draft_rows : 0, vocab);
   MOTIF_REQUIRE(workspace && workspace_bytes >= need, MOTIF_ERR_WORKSPACE,
                 "speculative_verify: workspace of %zu bytes, needs %zu", workspace_bytes, need);
   VerifyArgs a{};
@@ -264,11 +518,16 @@ int motif_speculative_verify(int dtype, const void* p_logits, int64_t p_batch_st
   a.path = path;
   a.next = next_token;
   a.T = (int)rows;
-  a.R = (int)draft_rows;
+  a.R = temperature == 0.0 ? 0 : (int)draft_rows;
   a.V = (int)vocab;
   a.inv_t = temperature > 0.0 ? 1.0 / temperature : 0.0;
-  MOTIF_DISPATCH_FLOAT(dtype, T, verify_kernel<T><<<(unsigned)batch, kVThreads, 0, as_stream(stream)>>>(a));
-  return check_launch("speculative_verify");
+  a.chunks = chunks_of(vocab);
+  a.stats = static_cast<float2*>(workspace);
+  a.tops = static_cast<unsigned long long*>(workspace);
+  MOTIF_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 8 == 0, MOTIF_ERR_BAD_CONTRACT,
+                "speculative_verify: workspace must be 8-byte aligned");
+  MOTIF_DISPATCH_FLOAT(dtype, T, return launch_verify<T>(a, batch, as_stream(stream)));
+  return MOTIF_OK;
 }
 
 }  // extern "C"

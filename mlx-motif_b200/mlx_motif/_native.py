@@ -159,7 +159,7 @@ SIGNATURES = {
         [_I, _I, _I, _P, _TKV, _P, _L, _F, _L, _L, _L, _L, _L, _L, _L, _P, _L, _P, _P, _S, _P, _P],
     ),
     "motif_kv4_keep_rows": (_I, [_I, _KV, _L, _P, _L, _P, _L, _L, _P, _L, _L, _P]),
-    "motif_speculative_verify_workspace_bytes": (_S, [_L, _L, _L]),
+    "motif_speculative_verify_workspace_bytes": (_S, [_L, _L, _L, _L]),
     "motif_speculative_verify": (
         _I,
         [_I, _P, _L, _L, _P, _L, _L, _L, _P, _P, _L, _P, _L, _L, _L, C.c_double, _P, _P, _P, _P, _S, _P],

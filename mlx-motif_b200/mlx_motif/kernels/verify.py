@@ -144,7 +144,7 @@ def speculative_verify(tokens: torch.Tensor, parents: torch.Tensor, p_logits: to
         q = _rows(q_logits) if sampled else None
         tok, par = contiguous(tokens), contiguous(parents)
         u = contiguous(uniforms) if sampled else None
-        ws_bytes = lib.motif_speculative_verify_workspace_bytes(B, T, R)
+        ws_bytes = lib.motif_speculative_verify_workspace_bytes(B, T, R, V)
         ws = workspace(ws_bytes, dev)
         check(lib.motif_speculative_verify(code, ptr(p), p.stride(0), p.stride(1), ptr(q), q.stride(0) if sampled else 0,
                                            q.stride(1) if sampled else 0, R, ptr(tok), ptr(par),
