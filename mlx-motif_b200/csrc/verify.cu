@@ -17,24 +17,25 @@
 //
 // Two launches:
 //   verify_stats_kernel reads every row once at memory speed: per 8192-entry chunk the maximum and Σ exp
-//     against it in 32 bits (the walk repeats a test that this cannot decide with sums in 64 bits), or at τ = 0 the largest logit and its first index;
+//     against it in 32 bits (the walk repeats a test that this cannot decide with sums in 64 bits), or at
+//     τ = 0 the largest logit and its first index;
 //   verify_walk_kernel walks the tree, one thread-block cluster a sequence. All CTAs of a cluster take the
 //     same decisions from the chunks' values; where a child is rejected they sum their parts of the row's
 //     S_j in 64 bits and exchange the sums through distributed shared memory (each part added in the same
 //     order by everyone, so the CTAs stay in step without another word). The draw finds the CTA, then the
 //     warp's range, then the entry.
 // The walk is bound by latency and by the 64-bit pipes: a pass over a row pair of 219520 entries is 439 k
-// exponentials of ~20 64-bit operations on the cluster's SMs.
+// exponentials of 11 64-bit operations on the cluster's SMs.
 #include <cooperative_groups.h>
 
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
 
 namespace motif {
 namespace {
-
 
 constexpr int kChunk = 8192, kStatThreads = 256;
 constexpr int kWalkThreads = 512, kWalkWarps = kWalkThreads / 32;
@@ -64,6 +65,28 @@ __device__ __forceinline__ float logit(const T* l, int i) {
 // exp((l − m)·inv_t); 1 at the maximum itself (infinite ones included), 0 for a row of −inf
 __device__ __forceinline__ double weight(float l, float m, double inv_t) {
   return m == -INFINITY ? 0.0 : l == m ? 1.0 : exp(((double)l - (double)m) * inv_t);
+}
+// The same for the sweeps over a row: e^x for x ≤ 0 by a table of 2^(j/64) (Tang, "Table-driven implementation
+// of the exponential function in IEEE floating-point arithmetic", ACM TOMS 15, 1989), x = (64k + j)·ln2/64 + r,
+// |r| ≤ 0.0055, the polynomial's first term left out r^6/720 < 4·10^-17; 11 64-bit operations. Below -708: 0.
+__device__ __forceinline__ double sweep_weight(float l, float m, double inv_t, const double* table) {
+  const double x = ((double)l - (double)m) * inv_t;
+  constexpr double kMagic = 6755399441055744.0;  // 1.5·2^52: the sum's low word is the rounded integer
+  const double t = fma(x, 92.332482616893656877, kMagic);  // 64 / ln 2
+  const int n = __double2loint(t);
+  const double nf = t - kMagic;
+  // ln2/64 = hi + lo, hi with 32 trailing zeros: nf·hi is exact
+  const double hi = __hiloint2double(0x3F862E42, 0);
+  const double lo = 0.010830424696249145 - hi;
+  const double r = fma(nf, -lo, fma(nf, -hi, x));
+  double p = fma(r, 1.0 / 120, 1.0 / 24);
+  p = fma(r, p, 1.0 / 6);
+  p = fma(r, p, 0.5);
+  p = fma(r, p, 1.0);
+  const double s = table[n & 63];
+  const double y = fma(s * r, p, s);
+  const double e = __hiloint2double(__double2hiint(y) + ((n >> 6) << 20), __double2loint(y));
+  return m == -INFINITY || !(x >= -708.0) ? (l == m && m != -INFINITY ? 1.0 : 0.0) : e;
 }
 
 // Order-preserving key of (value, index): the larger value, then the smaller index.
@@ -183,12 +206,14 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
 }
 
 // One cluster per sequence; CTA `rank` owns the vocabulary range [rank·V/C, (rank+1)·V/C), a warp a sixteenth of it.
-template <typename T>
+// CACHE: the range's exponentials of the current row pair fit shared memory and are computed once a row; else
+// every sweep computes them again.
+template <typename T, bool CACHE>
 __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyArgs a) {
   namespace cg = cooperative_groups;
   extern __shared__ __align__(16) uint8_t dyn[];
   __shared__ double ws[kWalkWarps], sums[2][kMaxCluster][2];
-  __shared__ double scan[kWalkWarps];
+  __shared__ double scan[kWalkWarps], table[64];
   __shared__ int found;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -203,9 +228,11 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyArgs a)
   float* qm = pm + a.T;
   double* pz = reinterpret_cast<double*>(dyn + ((7 * a.T * 4 + 15) & ~15));  // 1 / Σ
   double* qz = pz + a.T;
+  double* cache = qz + a.T;  // [2][range]: exponentials of the current row's target and draft
   const T* P = static_cast<const T*>(a.p) + b * a.pb;
   const T* Q = static_cast<const T*>(a.q) + b * a.qb;
   const bool greedy = a.inv_t == 0.0;
+  if (!greedy && tid < 64) table[tid] = exp2(tid / 64.0);
   for (int i = tid; i < a.T; i += kWalkThreads) {
     const int pa = i ? a.parents[b * a.parents_b + i] : -1, x = a.tokens[(int64_t)b * a.T + i];
     par[i] = pa;
@@ -301,17 +328,50 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyArgs a)
   bool exact = false;  // the laws' sums in 64 bits
   int32_t* path = a.path + (int64_t)b * a.T;
   if (rank == 0 && tid == 0) path[0] = 0;
-  auto wp = [&](const T* p, int e) { return weight(logit(p, e), lp.m, a.inv_t) * lp.inv_z; };
-  auto wq = [&](const T* q, int e) { return weight(logit(q, e), lq.m, a.inv_t) * lq.inv_z; };
-  auto make_exact = [&](const T* p, const T* q, bool with_q) {
-    double x = 0.0, y = 0.0, sx, sy;
-    for (int e = w0 + lane; e < w1; e += 32) {
-      x += weight(logit(p, e), lp.m, a.inv_t);
-      if (with_q) y += weight(logit(q, e), lq.m, a.inv_t);
+  const int span = v1 - v0;
+  // f(e, exp of p's entry, exp of q's) over my warp's range, entries of a lane 32 apart; several loads in flight.
+  // FILL computes and (CACHE) keeps the exponentials, else they come from the cache if there is one.
+  auto sweep = [&](const T* p, const T* q, auto fill, auto with_q, auto&& f) {
+    constexpr bool kFill = decltype(fill)::value, kQ = decltype(with_q)::value;
+    constexpr int kU = 8;
+    for (int e0 = w0 + lane; e0 < w1; e0 += 32 * kU) {
+      if constexpr (CACHE && !kFill) {
+#pragma unroll
+        for (int x = 0; x < kU; ++x) {
+          const int e = e0 + 32 * x;
+          if (e < w1) f(e, cache[e - v0], kQ ? cache[span + e - v0] : 0.0);
+        }
+      } else {
+        T lp_[kU], lq_[kU];
+#pragma unroll
+        for (int x = 0; x < kU; ++x) {
+          const int e = min(e0 + 32 * x, w1 - 1);
+          lp_[x] = p[e];
+          if (kQ) lq_[x] = q[e];
+        }
+#pragma unroll
+        for (int x = 0; x < kU; ++x) {
+          const int e = e0 + 32 * x;
+          const double ep = sweep_weight(logit(lp_, x), lp.m, a.inv_t, table);
+          const double eq = kQ ? sweep_weight(logit(lq_, x), lq.m, a.inv_t, table) : 0.0;
+          if (e >= w1) continue;
+          if constexpr (CACHE) {
+            cache[e - v0] = ep;
+            if (kQ) cache[span + e - v0] = eq;
+          }
+          f(e, ep, eq);
+        }
+      }
     }
+  };
+  constexpr std::true_type yes{};
+  constexpr std::false_type no{};
+  auto make_exact = [&](const T* p, const T* q) {
+    double x = 0.0, y = 0.0, sx, sy;
+    sweep(p, q, yes, yes, [&](int, double ep, double eq) { x += ep, y += eq; });
     total(x, y, sx, sy);
     lp.inv_z = sx > 0.0 ? 1.0 / sx : 0.0;
-    if (with_q) lq.inv_z = sy > 0.0 ? 1.0 / sy : 0.0;
+    lq.inv_z = sy > 0.0 ? 1.0 / sy : 0.0;
     exact = true;
   };
   for (int i = 1; i < a.T; ++i) {
@@ -323,7 +383,7 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyArgs a)
     if (!exact) lq = Law{qm[cur], qz[cur]};
     double pe = weight(px[i], lp.m, a.inv_t) * lp.inv_z, qe = weight(qx[i], lq.m, a.inv_t) * lq.inv_z;
     if (!exact && fabs((double)u[i] * qe * S - (pe - coef * qe)) <= kMargin * (pe + qe)) {
-      make_exact(p, q, true);
+      make_exact(p, q);
       pe = weight(px[i], lp.m, a.inv_t) * lp.inv_z, qe = weight(qx[i], lq.m, a.inv_t) * lq.inv_z;
     }
     if ((double)u[i] * qe * S < pe - coef * qe) {
@@ -334,24 +394,34 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyArgs a)
       lp = Law{pm[i], pz[i]};
       continue;
     }
-    if (!exact) make_exact(p, q, true);
+    if (!exact) make_exact(p, q);
     coef += S;
     double s = 0.0, unused;
-    for (int e = w0 + lane; e < w1; e += 32) s += fmax(0.0, wp(p, e) - coef * wq(q, e));
+    sweep(p, q, no, yes, [&](int, double ep, double eq) { s += fmax(0.0, ep * lp.inv_z - coef * (eq * lq.inv_z)); });
     total(s, 0.0, S, unused);
   }
   // the draw, from (p − coef·q)⁺ or (no rejection, or an empty residual) from p
   const T* p = P + cur * a.pr;
   const T* q = Q + (cur < a.R ? cur : 0) * a.qr;
   double W = S;
-  if (coef == 0.0 || !(S > 0.0)) {
-    coef = 0.0;
+  const bool plain = coef == 0.0 || !(S > 0.0);
+  if (plain) {
     double s = 0.0, unused;
-    for (int e = w0 + lane; e < w1; e += 32) s += weight(logit(p, e), lp.m, a.inv_t);
-    lp.inv_z = 1.0;
+    if (exact) sweep(p, q, no, no, [&](int, double ep, double) { s += ep; });
+    else sweep(p, q, yes, no, [&](int, double ep, double) { s += ep; });
     total(s, 0.0, W, unused);
   }
-  auto w = [&](int e) { return coef == 0.0 ? weight(logit(p, e), lp.m, a.inv_t) : fmax(0.0, wp(p, e) - coef * wq(q, e)); };
+  auto w = [&](int e) {
+    double ep, eq = 0.0;
+    if constexpr (CACHE) {
+      ep = cache[e - v0];
+      if (!plain) eq = cache[span + e - v0];
+    } else {
+      ep = sweep_weight(logit(p, e), lp.m, a.inv_t, table);
+      if (!plain) eq = sweep_weight(logit(q, e), lq.m, a.inv_t, table);
+    }
+    return plain ? ep : fmax(0.0, ep * lp.inv_z - coef * (eq * lq.inv_z));
+  };
   // the CTA, then the warp's range that holds the border; the last one with any weight if rounding leaves none beyond it
   const double target = (double)u[0] * W;
   double before = 0.0;
@@ -432,9 +502,14 @@ int launch_verify(const VerifyArgs& a, int64_t batch, cudaStream_t st) {
   // CTAs of a cluster: all SMs together serve the batch, and a CTA has 2048 entries or more
   int C = 1;
   while (!greedy && C < kMaxCluster && 2 * C * batch <= 128 && a.V / (2 * C) >= 2048) C *= 2;
-  auto kern = verify_walk_kernel<T>;
-  const size_t smem = ((7 * (size_t)a.T * 4 + 15) & ~(size_t)15) + 2 * (size_t)a.T * 8;
+  const size_t rows = ((7 * (size_t)a.T * 4 + 15) & ~(size_t)15) + 2 * (size_t)a.T * 8;
+  auto bytes = [&](int c) { return rows + 16 * (size_t)(a.V / c + 1); };
+  constexpr size_t kRoom = 224 * 1024;
+  bool cache = !greedy && bytes(C) <= kRoom;
+  auto kern = cache ? verify_walk_kernel<T, true> : verify_walk_kernel<T, false>;
+  size_t smem = cache ? bytes(C) : rows;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return fail(MOTIF_ERR_CUDA, "speculative_verify: cluster attribute: %s", cudaGetErrorString(e));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(batch * C));
@@ -460,6 +535,11 @@ int launch_verify(const VerifyArgs& a, int64_t batch, cudaStream_t st) {
       C = 8;
       cfg.gridDim = dim3((unsigned)(batch * C));
       at[1].val.clusterDim.x = 8;
+      cache = bytes(C) <= kRoom;
+      kern = cache ? verify_walk_kernel<T, true> : verify_walk_kernel<T, false>;
+      cfg.dynamicSmemBytes = smem = cache ? bytes(C) : rows;
+      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+      if (e != cudaSuccess) return fail(MOTIF_ERR_CUDA, "speculative_verify: %s", cudaGetErrorString(e));
     }
   }
   e = cudaLaunchKernelEx(&cfg, kern, a);
