@@ -59,8 +59,12 @@ struct VerifyArgs {
 
 template <typename T>
 __device__ __forceinline__ float logit(const T* l, int i) {
-  const float v = to_f<T>(l[i]);
-  return isnan(v) ? -INFINITY : v;
+  return fmaxf(to_f<T>(l[i]), -INFINITY);  // NaN counts as -inf
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 // exp((l − m)·inv_t); 1 at the maximum itself (infinite ones included), 0 for a row of −inf
 __device__ __forceinline__ double weight(float l, float m, double inv_t) {
@@ -170,17 +174,28 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(VerifyArgs a
 #pragma unroll
   for (int w = 0; w < 8; ++w) m = fmaxf(m, sf[w]);
   const float k = (float)a.inv_t * 1.4426950408889634f;
-  auto term = [&](float f) { return f == m ? 1.f : exp2f((f - m) * k); };  // m may be infinite
-  float z = edge >= 0 && m > -INFINITY ? term(ev) : 0.f;
-  if (m > -INFINITY) {
+  float z = 0.f;
+  if (m == INFINITY) {  // the infinite entries share the law
+    z = ev == m ? 1.f : 0.f;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int v = tid + i * kStatThreads;
       if (v >= n_vec) continue;
       const T* e = reinterpret_cast<const T*>(&raw[i]);
 #pragma unroll
-      for (int x = 0; x < kVec; ++x) z += term(logit(e, x));
+      for (int x = 0; x < kVec; ++x) z += to_f<T>(e[x]) == m ? 1.f : 0.f;
     }
+  } else if (m > -INFINITY) {
+    float zs[4] = {edge >= 0 ? ex2((ev - m) * k) : 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int v = tid + i * kStatThreads;
+      if (v >= n_vec) continue;
+      const T* e = reinterpret_cast<const T*>(&raw[i]);
+#pragma unroll
+      for (int x = 0; x < kVec; ++x) zs[x & 3] += ex2((logit(e, x) - m) * k);
+    }
+    z = (zs[0] + zs[1]) + (zs[2] + zs[3]);
   }
   z = warp_sum(z);
   __syncthreads();
@@ -333,7 +348,7 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyArgs a)
   // FILL computes and (CACHE) keeps the exponentials, else they come from the cache if there is one.
   auto sweep = [&](const T* p, const T* q, auto fill, auto with_q, auto&& f) {
     constexpr bool kFill = decltype(fill)::value, kQ = decltype(with_q)::value;
-    constexpr int kU = 8;
+    constexpr int kU = sizeof(T) == 2 ? 14 : 8;
     for (int e0 = w0 + lane; e0 < w1; e0 += 32 * kU) {
       if constexpr (CACHE && !kFill) {
 #pragma unroll
