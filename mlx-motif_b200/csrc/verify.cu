@@ -25,7 +25,7 @@
 //     order by everyone, so the CTAs stay in step without another word). The draw finds the CTA, then the
 //     warp's range, then the entry.
 // The walk is bound by latency and by the 64-bit pipes: a pass over a row pair of 219520 entries is 439 k
-// exponentials of 11 64-bit operations on the cluster's SMs.
+// exponentials of nine 64-bit operations on the cluster's SMs.
 #include <cooperative_groups.h>
 
 #include <atomic>
@@ -42,7 +42,7 @@ constexpr int kWalkThreads = 512, kWalkWarps = kWalkThreads / 32;
 constexpr int kMaxRows = 1024, kMaxCluster = 16;
 // The 32-bit row sums are within 2^-17 (exponent's rounding at |x| ≤ 60: 2^-18; 64 additions: 2^-18). A test closer
 // to its border than this is repeated with sums in 64 bits, both rows added in the same order.
-constexpr double kMargin = 1.0 / 32768;
+constexpr float kMargin = 1.f / 32768;
 
 struct VerifyArgs {
   const void *p, *q;
@@ -66,31 +66,24 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// exp((l − m)·inv_t); 1 at the maximum itself (infinite ones included), 0 for a row of −inf
-__device__ __forceinline__ double weight(float l, float m, double inv_t) {
-  return m == -INFINITY ? 0.0 : l == m ? 1.0 : exp(((double)l - (double)m) * inv_t);
-}
-// The same for the sweeps over a row: e^x for x ≤ 0 by a table of 2^(j/64) (Tang, "Table-driven implementation
-// of the exponential function in IEEE floating-point arithmetic", ACM TOMS 15, 1989), x = (64k + j)·ln2/64 + r,
-// |r| ≤ 0.0055, the polynomial's first term left out r^6/720 < 4·10^-17; 11 64-bit operations. Below -708: 0.
-__device__ __forceinline__ double sweep_weight(float l, float m, double inv_t, const double* table) {
-  const double x = ((double)l - (double)m) * inv_t;
-  constexpr double kMagic = 6755399441055744.0;  // 1.5·2^52: the sum's low word is the rounded integer
-  const double t = fma(x, 92.332482616893656877, kMagic);  // 64 / ln 2
+// exp((l − m)·inv_t) for the sweeps over a row, by a table of 2^(j/256) (Tang, "Table-driven implementation of the
+// exponential function in IEEE floating-point arithmetic", ACM TOMS 15, 1989): y = (l − m)·inv_t·log2 e =
+// n/256 + f, |f| ≤ 2^-9, 2^f by its series to f⁴ (the next term is 4·10^-17); nine 64-bit operations, within 2^-50
+// of exp for |y| ≤ 60 (y's own rounding). Below 2^-1022: 0. k = inv_t·log2 e, mk = m·k of a finite m.
+constexpr int kTable = 256;
+__device__ __forceinline__ double sweep_weight(float l, double k, double mk, const double* table) {
+  const double y = fma((double)l, k, -mk);
+  constexpr double kMagic = 6755399441055744.0 / kTable;  // 1.5·2^52 / 256: the sum rounds y to 1/256
+  const double t = y + kMagic;
   const int n = __double2loint(t);
-  const double nf = t - kMagic;
-  // ln2/64 = hi + lo, hi with 32 trailing zeros: nf·hi is exact
-  const double hi = __hiloint2double(0x3F862E42, 0);
-  const double lo = 0.010830424696249145 - hi;
-  const double r = fma(nf, -lo, fma(nf, -hi, x));
-  double p = fma(r, 1.0 / 120, 1.0 / 24);
-  p = fma(r, p, 1.0 / 6);
-  p = fma(r, p, 0.5);
-  p = fma(r, p, 1.0);
-  const double s = table[n & 63];
-  const double y = fma(s * r, p, s);
-  const double e = __hiloint2double(__double2hiint(y) + ((n >> 6) << 20), __double2loint(y));
-  return m == -INFINITY || !(x >= -708.0) ? (l == m && m != -INFINITY ? 1.0 : 0.0) : e;
+  const double f = y - (t - kMagic);
+  double q = fma(f, 0.0096181291076284772, 0.055504108664821580);  // (ln 2)^i / i!
+  q = fma(f, q, 0.24022650695910071);
+  q = fma(f, q, 0.69314718055994531);
+  const double s = table[n & (kTable - 1)];
+  const double e = fma(s * f, q, s);
+  const int hi = __double2hiint(e) + ((n >> 8) << 20);
+  return y >= -1022.0 ? __hiloint2double(hi, __double2loint(e)) : 0.0;
 }
 
 // Order-preserving key of (value, index): the larger value, then the smaller index.
@@ -209,58 +202,75 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(VerifyArgs a
   }
 }
 
-struct Law {
-  float m;
-  double inv_z;
-};
-
 __device__ __forceinline__ double warp_sum_f64(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
+// Bytes per tree row in shared memory: links, token, uniform, two logits, two probabilities, two laws (or a key).
+constexpr int kRowBytes = 4 * 12;
+
 // One cluster per sequence; CTA `rank` owns the vocabulary range [rank·V/C, (rank+1)·V/C), a warp a sixteenth of it.
 // CACHE: the range's exponentials of the current row pair fit shared memory and are computed once a row; else
-// every sweep computes them again.
+// every sweep computes them again. Most of the code runs once a call, so it is kept short: a line of it that is
+// not in the instruction cache costs as much as a load.
 template <typename T, bool CACHE>
 __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyArgs a) {
   namespace cg = cooperative_groups;
   extern __shared__ __align__(16) uint8_t dyn[];
   __shared__ double ws[kWalkWarps], sums[2][kMaxCluster][2];
-  __shared__ double scan[kWalkWarps], table[64];
+  __shared__ double scan[kWalkWarps], table[kTable];
   __shared__ int found;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int b = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // per tree row: parent, token, uniform; logits of its token in its parent's rows; laws of its own rows
-  int* par = reinterpret_cast<int*>(dyn);
+  const bool greedy = a.inv_t == 0.0;
+  unsigned long long* top = reinterpret_cast<unsigned long long*>(dyn);  // τ = 0: a row's largest entry; in place of …
+  float* pm = reinterpret_cast<float*>(dyn);                             // … the row's target law: maximum, 1 / Σ
+  float* pz = pm + a.T;
+  float* qm = pz + a.T;  // its draft law
+  float* qz = qm + a.T;
+  int* par = reinterpret_cast<int*>(qz + a.T);  // parent; -1: the root, or no row that can be accepted
   int* tok = par + a.T;
-  float* u = reinterpret_cast<float*>(tok + a.T);
-  float* px = u + a.T;
+  int* first = tok + a.T;  // first child, next sibling (-1: none)
+  int* next = first + a.T;
+  float* u = reinterpret_cast<float*>(next + a.T);
+  float* px = u + a.T;  // logits of the row's token in its parent's rows
   float* qx = px + a.T;
-  float* pm = qx + a.T;
-  float* qm = pm + a.T;
-  double* pz = reinterpret_cast<double*>(dyn + ((7 * a.T * 4 + 15) & ~15));  // 1 / Σ
-  double* qz = pz + a.T;
-  double* cache = qz + a.T;  // [2][range]: exponentials of the current row's target and draft
+  double* cache = reinterpret_cast<double*>(dyn + (((size_t)kRowBytes * a.T + 15) & ~(size_t)15));
   const T* P = static_cast<const T*>(a.p) + b * a.pb;
   const T* Q = static_cast<const T*>(a.q) + b * a.qb;
-  const bool greedy = a.inv_t == 0.0;
-  if (!greedy && tid < 64) table[tid] = exp2(tid / 64.0);
   for (int i = tid; i < a.T; i += kWalkThreads) {
-    const int pa = i ? a.parents[b * a.parents_b + i] : -1, x = a.tokens[(int64_t)b * a.T + i];
+    int pa = i ? a.parents[b * a.parents_b + i] : -1;
+    const int x = a.tokens[(int64_t)b * a.T + i];
+    if (pa >= i || x < 0 || x >= a.V || (!greedy && pa >= a.R)) pa = -1;
     par[i] = pa;
     tok[i] = x;
     if (greedy) continue;
     u[i] = a.u[(int64_t)b * a.T + i];
-    const bool test = pa >= 0 && pa < i && x >= 0 && x < a.V;
-    px[i] = test ? logit(P + pa * a.pr, x) : -INFINITY;
-    qx[i] = test && pa < a.R ? logit(Q + pa * a.qr, x) : -INFINITY;
+    px[i] = pa >= 0 ? logit(P + pa * a.pr, x) : 0.f;
+    qx[i] = pa >= 0 ? logit(Q + pa * a.qr, x) : 0.f;
+  }
+  if (!greedy && tid < kTable) table[tid] = exp2(tid / (double)kTable);
+  __syncthreads();
+  for (int i = tid; i < a.T; i += kWalkThreads) {
+    int f = -1, n = -1;
+    const int mine = par[i];
+#pragma unroll 1
+    for (int j = a.T - 1; j > i; --j) {
+      const int pj = par[j];
+      f = pj == i ? j : f;
+      n = pj == mine ? j : n;
+    }
+    first[i] = f;
+    next[i] = n;
   }
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
   // the rows' laws (τ = 0: their largest entries) from the chunks: eight lanes a row
-  for (int r0 = tid / 8; r0 < a.T + (greedy ? 0 : a.R); r0 += kWalkThreads / 8) {
+  const float kf = (float)a.inv_t * 1.4426950408889634f;
+#pragma unroll 1
+  for (int r0 = tid / 8; r0 < a.T + a.R; r0 += kWalkThreads / 8) {
     const unsigned mask = 0xFFu << (lane & 24);
     if (greedy) {
       unsigned long long k = 0;
@@ -273,53 +283,76 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyArgs a)
         const unsigned long long v = __shfl_xor_sync(mask, k, o);
         k = v > k ? v : k;
       }
-      if ((lane & 7) == 0) reinterpret_cast<unsigned long long*>(pz)[r0] = k;
+      if ((lane & 7) == 0) top[r0] = k;
       continue;
     }
     const float2* st = a.stats + ((int64_t)b * (a.T + a.R) + r0) * a.chunks;
-    float m = -INFINITY;
-    for (int c = lane & 7; c < a.chunks; c += 8) m = fmaxf(m, st[c].x);
+    float m = -INFINITY, z = 0.f;
+    for (int c0 = lane & 7; c0 < a.chunks; c0 += 32) {  // four chunks of a lane at once
+      float2 s[4];
 #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(mask, m, o));
-    double z = 0.0;
-    for (int c = lane & 7; c < a.chunks; c += 8) {
-      const float2 s = st[c];
-      z += s.x == m ? (double)s.y : s.x == -INFINITY ? 0.0 : (double)s.y * exp(((double)s.x - (double)m) * a.inv_t);
+      for (int x = 0; x < 4; ++x) s[x] = c0 + 8 * x < a.chunks ? st[c0 + 8 * x] : make_float2(-INFINITY, 0.f);
+      const float top4 = fmaxf(fmaxf(fmaxf(s[0].x, s[1].x), fmaxf(s[2].x, s[3].x)), m);
+      z = m == top4 ? z : z * ex2((m - top4) * kf);
+      m = top4;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) z += s[x].x == m ? s[x].y : s[x].y * ex2((s[x].x - m) * kf);
     }
 #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) z += __shfl_xor_sync(mask, z, o);
+    for (int o = 4; o > 0; o >>= 1) {
+      const float m2 = __shfl_xor_sync(mask, m, o), z2 = __shfl_xor_sync(mask, z, o), t = fmaxf(m, m2);
+      z = (m == t ? z : z * ex2((m - t) * kf)) + (m2 == t ? z2 : z2 * ex2((m2 - t) * kf));
+      m = t;
+    }
     if ((lane & 7) == 0) {
-      (r0 < a.T ? pm : qm)[r0 < a.T ? r0 : r0 - a.T] = m;
-      (r0 < a.T ? pz : qz)[r0 < a.T ? r0 : r0 - a.T] = m > -INFINITY && z > 0.0 ? 1.0 / z : 0.0;
+      const bool p = r0 < a.T;
+      const int r = p ? r0 : r0 - a.T;
+      (p ? pm : qm)[r] = m;
+      (p ? pz : qz)[r] = m > -INFINITY ? 1.f / z : 0.f;  // a row without a finite logit has no law
     }
   }
   __syncthreads();
 
+  int32_t* path = a.path + (int64_t)b * a.T;
   if (greedy) {
-    const unsigned long long* top = reinterpret_cast<const unsigned long long*>(pz);
     if (tid == 0) {
       int cur = 0, kept = 1;
       auto best = [&](int r) { return key_value(top[r]) > -INFINITY ? key_index(top[r]) : -1; };
       int want = best(0);
-      int32_t* path = a.path + (int64_t)b * a.T;
       path[0] = 0;
-      for (int i = 1; i < a.T; ++i)
-        if (par[i] == cur && want >= 0 && tok[i] == want) {
+      for (int i = first[0]; i >= 0;) {
+        if (want >= 0 && tok[i] == want) {
           cur = i;
           path[kept++] = i;
           want = best(i);
+          i = first[cur];
+        } else {
+          i = next[i];
         }
-      for (int i = kept; i < a.T; ++i) path[i] = -1;
+      }
       a.accepted[b] = kept - 1;
       a.next[b] = max(want, 0);
+      found = kept;
     }
+    __syncthreads();
+    for (int i = found + tid; i < a.T; i += kWalkThreads) path[i] = -1;
     return;
   }
 
-  const int v0 = (int)((int64_t)rank * a.V / C), v1 = (int)((int64_t)(rank + 1) * a.V / C);
-  auto range = [&](int w) { return v0 + (int)((int64_t)w * (v1 - v0) / kWalkWarps); };
+  const int v0 = (int)((int64_t)rank * a.V / C), v1 = (int)((int64_t)(rank + 1) * a.V / C), span = v1 - v0;
+  auto range = [&](int w) { return v0 + (int)((int64_t)w * span / kWalkWarps); };
   const int w0 = range(warp), w1 = range(warp + 1);
+  const double k = a.inv_t * 1.4426950408889634074;  // log2 e
+  // The current row's laws: maxima, and in `exact` form 1 / Σ in 64 bits; its residual (p − coef·q)⁺ / S.
+  float mp = pm[0], mq = 0.f;
+  double izp = 1.0, izq = 1.0, coef = 0.0, S = 1.0;
+  bool exact = false;
   int phase = 0;
+  // exp((l − m)/τ); an infinite maximum's entries share the law, a row of -inf has none
+  auto entry = [&](float l, float m) {
+    const double e = sweep_weight(l, k, (double)m * k, table);
+    return fabsf(m) < INFINITY ? e : m > 0.f && l == m ? 1.0 : 0.0;
+  };
   // Sums of two values over the cluster, the same on every CTA; my warps' sums of the first stay in ws.
   auto total = [&](double x, double y, double& sx, double& sy) {
     x = warp_sum_f64(x), y = warp_sum_f64(y);
@@ -328,92 +361,91 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyArgs a)
     __syncthreads();
     if (tid < C) {  // my CTA's sums into every CTA's slots
       double cx = 0.0, cy = 0.0;
+#pragma unroll 4
       for (int w = 0; w < kWalkWarps; ++w) cx += ws[w], cy += scan[w];
       double* dst = cluster.map_shared_rank(&sums[phase][rank][0], tid);
       dst[0] = cx, dst[1] = cy;
     }
     cluster.sync();
     sx = sy = 0.0;
+#pragma unroll 4
     for (int c = 0; c < C; ++c) sx += sums[phase][c][0], sy += sums[phase][c][1];
     phase ^= 1;  // the other slots' readers are behind the next sync
   };
-  int cur = 0, kept = 1;
-  double coef = 0.0, S = 1.0;
-  Law lp{pm[0], pz[0]}, lq{};
-  bool exact = false;  // the laws' sums in 64 bits
-  int32_t* path = a.path + (int64_t)b * a.T;
-  if (rank == 0 && tid == 0) path[0] = 0;
-  const int span = v1 - v0;
-  // f(e, exp of p's entry, exp of q's) over my warp's range, entries of a lane 32 apart; several loads in flight.
-  // FILL computes and (CACHE) keeps the exponentials, else they come from the cache if there is one.
-  auto sweep = [&](const T* p, const T* q, auto fill, auto with_q, auto&& f) {
-    constexpr bool kFill = decltype(fill)::value, kQ = decltype(with_q)::value;
-    constexpr int kU = sizeof(T) == 2 ? 14 : 8;
+  // Exponentials of my warp's range of the row(s) into the cache: the logits first, many loads in flight, then each
+  // in place of its logit.
+  auto fill = [&](const T* p, const T* q) {
+    constexpr int kU = 9;
     for (int e0 = w0 + lane; e0 < w1; e0 += 32 * kU) {
-      if constexpr (CACHE && !kFill) {
+      T x[kU], y[kU];
 #pragma unroll
-        for (int x = 0; x < kU; ++x) {
-          const int e = e0 + 32 * x;
-          if (e < w1) f(e, cache[e - v0], kQ ? cache[span + e - v0] : 0.0);
-        }
-      } else {
-        T lp_[kU], lq_[kU];
+      for (int i = 0; i < kU; ++i) {
+        const int e = min(e0 + 32 * i, w1 - 1);
+        x[i] = p[e];
+        if (q) y[i] = q[e];
+      }
 #pragma unroll
-        for (int x = 0; x < kU; ++x) {
-          const int e = min(e0 + 32 * x, w1 - 1);
-          lp_[x] = p[e];
-          if (kQ) lq_[x] = q[e];
-        }
-#pragma unroll
-        for (int x = 0; x < kU; ++x) {
-          const int e = e0 + 32 * x;
-          const double ep = sweep_weight(logit(lp_, x), lp.m, a.inv_t, table);
-          const double eq = kQ ? sweep_weight(logit(lq_, x), lq.m, a.inv_t, table) : 0.0;
-          if (e >= w1) continue;
-          if constexpr (CACHE) {
-            cache[e - v0] = ep;
-            if (kQ) cache[span + e - v0] = eq;
-          }
-          f(e, ep, eq);
-        }
+      for (int i = 0; i < kU; ++i) {
+        const int e = min(e0 + 32 * i, w1 - 1);  // the last lanes write one entry more than once, the same value
+        *reinterpret_cast<float*>(cache + e - v0) = logit(x, i);
+        if (q) *reinterpret_cast<float*>(cache + span + e - v0) = logit(y, i);
       }
     }
+    __syncwarp();
+#pragma unroll 4
+    for (int e = w0 + lane - v0; e < w1 - v0; e += 32) {
+      cache[e] = entry(*reinterpret_cast<const float*>(cache + e), mp);
+      if (q) cache[span + e] = entry(*reinterpret_cast<const float*>(cache + span + e), mq);
+    }
+    __syncwarp();
   };
-  constexpr std::true_type yes{};
-  constexpr std::false_type no{};
+  auto at_p = [&](const T* p, int e) { return CACHE ? cache[e - v0] : entry(logit(p, e), mp); };
+  auto at_q = [&](const T* q, int e) { return CACHE ? cache[span + e - v0] : entry(logit(q, e), mq); };
   auto make_exact = [&](const T* p, const T* q) {
+    if (CACHE) fill(p, q);
     double x = 0.0, y = 0.0, sx, sy;
-    sweep(p, q, yes, yes, [&](int, double ep, double eq) { x += ep, y += eq; });
+#pragma unroll 4
+    for (int e = w0 + lane; e < w1; e += 32) x += at_p(p, e), y += at_q(q, e);
     total(x, y, sx, sy);
-    lp.inv_z = sx > 0.0 ? 1.0 / sx : 0.0;
-    lq.inv_z = sy > 0.0 ? 1.0 / sy : 0.0;
+    izp = sx > 0.0 ? 1.0 / sx : 0.0;
+    izq = sy > 0.0 ? 1.0 / sy : 0.0;
     exact = true;
   };
-  for (int i = 1; i < a.T; ++i) {
-    if (par[i] != cur) continue;
-    const int x = tok[i];
-    if (x < 0 || x >= a.V || cur >= a.R) continue;  // a padding row; a row without a draft row
+
+  int cur = 0, kept = 1;
+  if (rank == 0 && tid == 0) path[0] = 0;
+  for (int i = first[0]; i >= 0;) {
     const T* p = P + cur * a.pr;
     const T* q = Q + cur * a.qr;
-    if (!exact) lq = Law{qm[cur], qz[cur]};
-    double pe = weight(px[i], lp.m, a.inv_t) * lp.inv_z, qe = weight(qx[i], lq.m, a.inv_t) * lq.inv_z;
-    if (!exact && fabs((double)u[i] * qe * S - (pe - coef * qe)) <= kMargin * (pe + qe)) {
-      make_exact(p, q);
-      pe = weight(px[i], lp.m, a.inv_t) * lp.inv_z, qe = weight(qx[i], lq.m, a.inv_t) * lq.inv_z;
+    bool ok = false, sure = false;
+    if (!exact) {  // the first child: w = p, in 32 bits where that decides
+      mq = qm[cur];
+      auto prob = [&](float l, float m, float iz) { return l == m ? iz : ex2((l - m) * kf) * iz; };
+      const float pe = prob(px[i], mp, pz[cur]), qe = prob(qx[i], mq, qz[cur]), ue = u[i] * qe;
+      ok = ue < pe;
+      sure = fabsf(ue - pe) > kMargin * (pe + qe);
     }
-    if ((double)u[i] * qe * S < pe - coef * qe) {
+    if (!sure) {
+      if (!exact) make_exact(p, q);
+      const double pe = entry(px[i], mp) * izp, qe = entry(qx[i], mq) * izq;
+      ok = (double)u[i] * qe * S < pe - coef * qe;
+    }
+    if (ok) {
       if (rank == 0 && tid == 0) path[kept] = i;
       ++kept;
       cur = i;
+      i = first[cur];
       coef = 0.0, S = 1.0, exact = false;
-      lp = Law{pm[i], pz[i]};
+      mp = pm[cur];
       continue;
     }
     if (!exact) make_exact(p, q);
     coef += S;
     double s = 0.0, unused;
-    sweep(p, q, no, yes, [&](int, double ep, double eq) { s += fmax(0.0, ep * lp.inv_z - coef * (eq * lq.inv_z)); });
+#pragma unroll 4
+    for (int e = w0 + lane; e < w1; e += 32) s += fmax(0.0, at_p(p, e) * izp - coef * (at_q(q, e) * izq));
     total(s, 0.0, S, unused);
+    i = next[i];
   }
   // the draw, from (p − coef·q)⁺ or (no rejection, or an empty residual) from p
   const T* p = P + cur * a.pr;
@@ -422,21 +454,12 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyArgs a)
   const bool plain = coef == 0.0 || !(S > 0.0);
   if (plain) {
     double s = 0.0, unused;
-    if (exact) sweep(p, q, no, no, [&](int, double ep, double) { s += ep; });
-    else sweep(p, q, yes, no, [&](int, double ep, double) { s += ep; });
+    if (CACHE && !exact) fill(p, nullptr);
+#pragma unroll 4
+    for (int e = w0 + lane; e < w1; e += 32) s += at_p(p, e);
     total(s, 0.0, W, unused);
   }
-  auto w = [&](int e) {
-    double ep, eq = 0.0;
-    if constexpr (CACHE) {
-      ep = cache[e - v0];
-      if (!plain) eq = cache[span + e - v0];
-    } else {
-      ep = sweep_weight(logit(p, e), lp.m, a.inv_t, table);
-      if (!plain) eq = sweep_weight(logit(q, e), lq.m, a.inv_t, table);
-    }
-    return plain ? ep : fmax(0.0, ep * lp.inv_z - coef * (eq * lq.inv_z));
-  };
+  auto w = [&](int e) { return plain ? at_p(p, e) : fmax(0.0, at_p(p, e) * izp - coef * (at_q(q, e) * izq)); };
   // the CTA, then the warp's range that holds the border; the last one with any weight if rounding leaves none beyond it
   const double target = (double)u[0] * W;
   double before = 0.0;
@@ -503,7 +526,7 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyArgs a)
     if (tid == 0) a.accepted[b] = kept - 1;
     for (int i = kept + tid; i < a.T; i += kWalkThreads) path[i] = -1;
   }
-  cluster.sync();  // no CTA ends while another may still write into its shared memory
+  // every write into another CTA's shared memory was before the last sync: a CTA may end
 }
 
 int chunks_of(int64_t V) { return (int)ceil_div(V, kChunk); }
@@ -517,7 +540,7 @@ int launch_verify(const VerifyArgs& a, int64_t batch, cudaStream_t st) {
   // CTAs of a cluster: all SMs together serve the batch, and a CTA has 2048 entries or more
   int C = 1;
   while (!greedy && C < kMaxCluster && 2 * C * batch <= 128 && a.V / (2 * C) >= 2048) C *= 2;
-  const size_t rows = ((7 * (size_t)a.T * 4 + 15) & ~(size_t)15) + 2 * (size_t)a.T * 8;
+  const size_t rows = ((size_t)kRowBytes * a.T + 15) & ~(size_t)15;
   auto bytes = [&](int c) { return rows + 16 * (size_t)(a.V / c + 1); };
   constexpr size_t kRoom = 224 * 1024;
   bool cache = !greedy && bytes(C) <= kRoom;
