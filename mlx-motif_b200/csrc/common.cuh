@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "motif_b200.h"
@@ -18,6 +19,19 @@ int check_launch(const char* what);
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Runs `set` (a kernel's attributes) once per device and caller's `done` word; `set` returns a cudaError_t.
+template <typename F>
+inline cudaError_t once_per_device(std::atomic<uint64_t>& done, F&& set) {
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+  const cudaError_t r = set();
+  if (r == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_release);
+  return r;
+}
 
 // ---- dtype traits ------------------------------------------------------------
 template <typename T>

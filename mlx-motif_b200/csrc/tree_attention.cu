@@ -1192,10 +1192,17 @@ __global__ void __launch_bounds__(32 * kMergeWarps * kMergeRows) tree_merge_kern
   }
 }
 
-int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+int sm_count() {  // of the first device asked for: a machine's GPUs are alike
+  static std::atomic<int> known{0};
+  int n = known;
+  if (n > 0) return n;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
+      n < 1) {
+    (void)cudaGetLastError();
     return 148;
+  }
+  known = n;
   return n;
 }
 
@@ -1266,7 +1273,9 @@ int launch_merge(const TreeArgs& a, const Plan& p, cudaStream_t st) {
 template <typename T, int D, int BITS>
 int launch_simt(const TreeArgs& a, const Plan& p, cudaStream_t st) {
   auto kern = tree_simt_kernel<T, D, BITS>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, simt_smem<D>());
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = once_per_device(
+      done, [&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, simt_smem<D>()); });
   if (e != cudaSuccess) return fail(MOTIF_ERR_CUDA, "sdpa_dual_v_tree: smem attribute: %s", cudaGetErrorString(e));
   kern<<<grid_of(a, p), kSThreads, simt_smem<D>(), st>>>(a);
   const int rc = check_launch("sdpa_dual_v_tree");
@@ -1295,7 +1304,9 @@ int launch_tc(const TreeArgs& a, const Plan& p, cudaStream_t st) {
     smem += ta.raw_stages * raw;
   }
   auto kern = tree_tc_kernel<T, D, BITS>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<uint64_t> done{0};  // the most that any group size takes
+  const cudaError_t e = once_per_device(
+      done, [&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024); });
   if (e != cudaSuccess) return fail(MOTIF_ERR_CUDA, "sdpa_dual_v_tree: smem attribute: %s", cudaGetErrorString(e));
   kern<<<grid_of(a, p), TcCfg<BITS>::kThreads, smem, st>>>(ta);
   const int rc = check_launch("sdpa_dual_v_tree");

@@ -529,6 +529,8 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyArgs a)
   // every write into another CTA's shared memory was before the last sync: a CTA may end
 }
 
+constexpr size_t kRoom = 224 * 1024;  // dynamic shared memory beside the walk's static 2.8 KB
+
 int chunks_of(int64_t V) { return (int)ceil_div(V, kChunk); }
 
 template <typename T>
@@ -542,17 +544,22 @@ int launch_verify(const VerifyArgs& a, int64_t batch, cudaStream_t st) {
   while (!greedy && C < kMaxCluster && 2 * C * batch <= 128 && a.V / (2 * C) >= 2048) C *= 2;
   const size_t rows = ((size_t)kRowBytes * a.T + 15) & ~(size_t)15;
   auto bytes = [&](int c) { return rows + 16 * (size_t)(a.V / c + 1); };
-  constexpr size_t kRoom = 224 * 1024;
   bool cache = !greedy && bytes(C) <= kRoom;
   auto kern = cache ? verify_walk_kernel<T, true> : verify_walk_kernel<T, false>;
-  size_t smem = cache ? bytes(C) : rows;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = once_per_device(done, [] {
+    for (auto f : {verify_walk_kernel<T, true>, verify_walk_kernel<T, false>}) {
+      cudaError_t r = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (r == cudaSuccess) r = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRoom);
+      if (r != cudaSuccess) return r;
+    }
+    return cudaSuccess;
+  });
   if (e != cudaSuccess) return fail(MOTIF_ERR_CUDA, "speculative_verify: cluster attribute: %s", cudaGetErrorString(e));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(batch * C));
   cfg.blockDim = dim3(kWalkThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = cache ? bytes(C) : rows;
   cfg.stream = st;
   cudaLaunchAttribute at[2]{};
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -575,9 +582,7 @@ int launch_verify(const VerifyArgs& a, int64_t batch, cudaStream_t st) {
       at[1].val.clusterDim.x = 8;
       cache = bytes(C) <= kRoom;
       kern = cache ? verify_walk_kernel<T, true> : verify_walk_kernel<T, false>;
-      cfg.dynamicSmemBytes = smem = cache ? bytes(C) : rows;
-      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-      if (e != cudaSuccess) return fail(MOTIF_ERR_CUDA, "speculative_verify: %s", cudaGetErrorString(e));
+      cfg.dynamicSmemBytes = cache ? bytes(C) : rows;
     }
   }
   e = cudaLaunchKernelEx(&cfg, kern, a);

@@ -8,8 +8,9 @@ causal prompt blocks; same shapes, runtime ``kv_len`` and assertion style as the
 
 from __future__ import annotations
 
-import ctypes as C
+import functools
 import math
+import struct
 
 import torch
 
@@ -132,33 +133,38 @@ def _check_device(t: torch.Tensor, device) -> None:
         raise ValueError(f"tensors on {t.device} and {device}: all operands must be on one CUDA device")
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(device_index, *shape) -> int:
+    return lib.motif_sdpa_dual_v_tree_workspace_bytes(*shape)
+
+
 def _launch(q, parts, strides, bits, group_size, scale, HKV, cap, kv_len, tree_mask, name):
-    """parts: the (data, scales, biases) of k, v1, v2 (scales and biases None for plain rows)."""
+    """parts: data, scales, biases of k, v1, v2 in turn (scales and biases None for plain rows)."""
     B, HQ, T, D = q.shape
     dev = q.device
     code = dtype_code(q)
-    for part in parts:
-        for t in part:
-            if t is not None:
-                _check_device(t, dev)
+    for t in parts:
+        if t is not None and t.device != dev:
+            _check_device(t, dev)
     n, n_dev, n_step = _check_len(kv_len, B, T, cap, dev)
     mask, mask_b = _check_mask(tree_mask, B, T, dev)
     y = torch.empty((B, HQ, T, 2 * D), dtype=q.dtype, device=dev)
     if B == 0 or cap == 0:
         return y.zero_()
-    kv = motif_tree_kv()
-    for i, (data, scales, biases) in enumerate(parts):
-        kv.data[i], kv.scales[i], kv.biases[i] = ptr(data), ptr(scales), ptr(biases)
-    kv.stride[0], kv.stride[1], kv.stride[2] = strides
     with on_device(dev):
         qc = _aligned(q)
-        ws_bytes = lib.motif_sdpa_dual_v_tree_workspace_bytes(code, bits, group_size, B, HQ, HKV, T, cap, D,
-                                                              cap if n_dev else n, 1 - n_step)
+        # motif_tree_kv: data[3], scales[3], biases[3], stride[3]
+        at = [0 if t is None else t.data_ptr() for t in parts]
+        kv = motif_tree_kv.from_buffer_copy(_KV.pack(*at[0::3], *at[1::3], *at[2::3], *strides))
+        ws_bytes = _workspace_bytes(dev.index, code, bits, group_size, B, HQ, HKV, T, cap, D, cap if n_dev else n, 1 - n_step)
         ws = workspace(ws_bytes, dev)
-        check(lib.motif_sdpa_dual_v_tree(code, bits, group_size, ptr(qc), C.byref(kv), ptr(mask), mask_b, float(scale),
-                                         B, HQ, HKV, T, cap, D, n, n_dev, n_step, ptr(y), ptr(ws), ws_bytes, None,
+        check(lib.motif_sdpa_dual_v_tree(code, bits, group_size, qc.data_ptr(), kv, ptr(mask), mask_b, float(scale), B, HQ,
+                                         HKV, T, cap, D, n, n_dev, n_step, y.data_ptr(), ws.data_ptr(), ws_bytes, None,
                                          stream(dev)), name)
     return y
+
+
+_KV = struct.Struct("12q")
 
 
 def sdpa_dual_v_tree(q: torch.Tensor, k: torch.Tensor, v1: torch.Tensor, v2: torch.Tensor, scale: float, kv_len=None,
@@ -176,12 +182,13 @@ def sdpa_dual_v_tree(q: torch.Tensor, k: torch.Tensor, v1: torch.Tensor, v2: tor
         return sdpa_dual_v_tree_reference(q, k, v1, v2, scale, kv_len, tree_mask)
     B, HQ, T, D, HKV, cap = _check_q(q, k.shape, "sdpa_dual_v_tree")
     assert k.shape == v1.shape == v2.shape == (B, HKV, cap, D), "k, v1, v2 must match (B, H_kv, KV_cap, D)"
-    rows = [t.to(q.dtype) for t in (k, v1, v2)]
-    strides = _row_strides(rows[0])
-    if strides is None or any(_row_strides(t) != strides for t in rows[1:]):
-        rows = [_aligned(t) for t in rows]
-        strides = _row_strides(rows[0]) if cap else (0, 0, 0)
-    return _launch(q, [(t, None, None) for t in rows], strides, 16, 64, scale, HKV, cap, kv_len, tree_mask,
+    if not k.dtype == v1.dtype == v2.dtype == q.dtype:
+        k, v1, v2 = (t.to(q.dtype) for t in (k, v1, v2))
+    strides = _row_strides(k)
+    if strides is None or _row_strides(v1) != strides or _row_strides(v2) != strides:
+        k, v1, v2 = (_aligned(t) for t in (k, v1, v2))
+        strides = _row_strides(k) if cap else (0, 0, 0)
+    return _launch(q, (k, None, None, v1, None, None, v2, None, None), strides, 16, 64, scale, HKV, cap, kv_len, tree_mask,
                    "sdpa_dual_v_tree")
 
 
@@ -204,5 +211,5 @@ def sdpa_dual_v_tree_q4(q: torch.Tensor, k_q: tuple, v1_q: tuple, v2_q: tuple, s
             "scales and biases must match (B, H_kv, KV_cap, D/group_size)"
         if data.dtype not in (torch.uint32, torch.int32):
             raise TypeError(f"packed data must be uint32, got {data.dtype}")
-        parts.append([_aligned(t) for t in (data, scales.to(q.dtype), biases.to(q.dtype))])
+        parts += [_aligned(t) for t in (data, scales.to(q.dtype), biases.to(q.dtype))]
     return _launch(q, parts, (0, 0, 0), bits, int(group_size), scale, HKV, cap, kv_len, tree_mask, "sdpa_dual_v_tree_q4")

@@ -8,6 +8,7 @@ its own numbers for one chain.
 
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple
 
@@ -85,6 +86,11 @@ def speculative_verify_reference(tokens, parents, p_logits, q_logits, uniforms, 
                         torch.tensor(nxt, dtype=torch.int32, device=dev))
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(*shape) -> int:
+    return lib.motif_speculative_verify_workspace_bytes(*shape)
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """Logits whose vocabulary axis is contiguous (batch and row strides are passed on)."""
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
@@ -135,8 +141,8 @@ def speculative_verify(tokens: torch.Tensor, parents: torch.Tensor, p_logits: to
     for t in (tokens, parents) + ((q_logits, uniforms) if sampled else ()):
         if t.device != dev:
             raise ValueError(f"tensors on {t.device} and {dev}: all operands must be on one CUDA device")
-    out = VerifyResult(torch.empty(B, dtype=torch.int32, device=dev), torch.empty((B, T), dtype=torch.int32, device=dev),
-                       torch.empty(B, dtype=torch.int32, device=dev))
+    both = torch.empty((2, B), dtype=torch.int32, device=dev)  # one allocation for the counts and the tokens
+    out = VerifyResult(both[0], torch.empty((B, T), dtype=torch.int32, device=dev), both[1])
     if B == 0:
         return out
     with on_device(dev):
@@ -144,11 +150,12 @@ def speculative_verify(tokens: torch.Tensor, parents: torch.Tensor, p_logits: to
         q = _rows(q_logits) if sampled else None
         tok, par = contiguous(tokens), contiguous(parents)
         u = contiguous(uniforms) if sampled else None
-        ws_bytes = lib.motif_speculative_verify_workspace_bytes(B, T, R, V)
+        ws_bytes = _workspace_bytes(B, T, R, V)
         ws = workspace(ws_bytes, dev)
-        check(lib.motif_speculative_verify(code, ptr(p), p.stride(0), p.stride(1), ptr(q), q.stride(0) if sampled else 0,
-                                           q.stride(1) if sampled else 0, R, ptr(tok), ptr(par),
+        pb, pr, _ = p.stride()
+        qb, qr, _ = q.stride() if sampled else (0, 0, 0)
+        check(lib.motif_speculative_verify(code, p.data_ptr(), pb, pr, ptr(q), qb, qr, R, tok.data_ptr(), par.data_ptr(),
                                            T if parents.dim() == 2 else 0, ptr(u), B, T, V, temperature,
-                                           ptr(out.accepted), ptr(out.path), ptr(out.next_token), ptr(ws), ws_bytes,
-                                           stream(dev)), "speculative_verify")
+                                           out.accepted.data_ptr(), out.path.data_ptr(), out.next_token.data_ptr(),
+                                           ws.data_ptr(), ws_bytes, stream(dev)), "speculative_verify")
     return out
