@@ -383,8 +383,10 @@ constexpr int kTR = 128, kTK = 64;
 
 template <int BITS>
 struct TcCfg {
-  static constexpr int kStages = BITS == 16 ? 3 : 2;   // K operand tiles
-  static constexpr int kVStages = BITS == 16 ? 4 : 2;  // V operand tiles: held until P·V, while K is free after S
+  // K and V operand tiles. V is held until P·V, K free after S; packed caches also need room for raw tiles
+  // (8-bit ones are twice as large).
+  static constexpr int kStages = BITS == 8 ? 2 : 3;
+  static constexpr int kVStages = BITS == 16 ? 4 : BITS == 4 ? 3 : 2;
   static constexpr int kThreads = BITS == 16 ? 320 : 512;
   static constexpr int kFill = BITS == 16 ? 1 : 6;  // arrivals that fill a K or V tile
 };
@@ -828,7 +830,7 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
         const uint32_t ts = trow + kColS + kTK * (it % kSBufs);
         bool need = false;
         float factor = 1.f, mb = 0.f, mul = mult;
-        constexpr bool kKeep = BITS == 16;  // registers for all 64 columns; else they are read twice
+        constexpr bool kKeep = BITS == 16;  // registers for all 64 columns; else they are read twice, in one loop's code
         float sv[kKeep ? 2 : 1][32];
         auto load_s = [&](int h, float (&x)[32]) {
           uint32_t u[32];
@@ -850,7 +852,7 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
         if (work) {
           if (tail) mul = 1.f;
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
+#pragma unroll(kKeep ? 2 : 1)
           for (int h = 0; h < 2; ++h) {
             load_s(h, sv[kKeep ? h : 0]);
 #pragma unroll
@@ -913,7 +915,7 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
         }
         if (work) {  // P in the type (one rounding of each weight), over the first half of its S
           float ps[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
+#pragma unroll(kKeep ? 2 : 1)
           for (int h = 0; h < 2; ++h) {
             float(&x)[32] = sv[kKeep ? h : 0];
             if constexpr (!kKeep) load_s(h, x);
@@ -1015,6 +1017,8 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
     const int tid = threadIdx.x - 320;
     const int gs_log = 31 - __clz(a.gs);  // the group size divides 64 or 128
     constexpr int kUnits = kTK * D / 32;  // 32 channels of one row
+    constexpr int kFillThreads = Cfg::kThreads - 320, kPer = 3 * kUnits / kFillThreads;
+    static_assert(kPer * kFillThreads == 3 * kUnits, "whole units per thread");
     int it = 0;
     bool alive = true;
     for (; alive && more; more = sched.next(a, sg)) {
@@ -1025,19 +1029,28 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
                         (it < NS || (bar_wait(k_empty(s), par) && bar_wait(v_empty(s), par)));  // NV is NS here
         if (__any_sync(0xffffffffu, !ok || *abort_flag)) { alive = false; break; }
         const uint8_t* raw = smem + Map::kRaw + rs * (3 * kTK * ta.code_bytes + 6 * kTK * ta.group_bytes);
-        for (int u = tid; u < 3 * kUnits; u += Cfg::kThreads - 320) {  // 3·kUnits is a multiple of the threads
-          const int slot = u / kUnits, row = u % kUnits / (D / 32), c32 = u % (D / 32);
-          const uint8_t* codes = raw + (slot * kTK + row) * ta.code_bytes + c32 * BITS * 4;
-          const uint8_t* scales = raw + 3 * kTK * ta.code_bytes + (slot * 2 * kTK + row) * ta.group_bytes;
-          uint8_t* tile = smem + (slot == 0 ? Map::kK + s * Map::kKBytes : Map::kV + s * Map::kVBytes + (slot - 1) * Map::kKBytes);
+        // One short loop (several roles' code shares the instruction caches), the next unit's codes on their way.
+        auto unit = [&](int x, uint32_t (&w)[BITS], int& at, const T*& sc, uint8_t*& tile) {
+          const int u = tid + x * kFillThreads, slot = u / kUnits, row = u % kUnits / (D / 32), c32 = u % (D / 32);
+          const uint4* codes = reinterpret_cast<const uint4*>(raw + (slot * kTK + row) * ta.code_bytes + c32 * BITS * 4);
+#pragma unroll
+          for (int i = 0; i < BITS / 4; ++i) *reinterpret_cast<uint4*>(w + 4 * i) = codes[i];
+          sc = reinterpret_cast<const T*>(raw + 3 * kTK * ta.code_bytes + (slot * 2 * kTK + row) * ta.group_bytes);
+          tile = smem + (slot == 0 ? Map::kK + s * Map::kKBytes : Map::kV + s * Map::kVBytes + (slot - 1) * Map::kKBytes) + row * 128;
+          at = row << 8 | c32;
+        };
+        uint32_t w[BITS], w2[BITS];
+        int at, at2;
+        const T *sc, *sc2;
+        uint8_t *tile, *tile2;
+        unit(0, w, at, sc, tile);
+#pragma unroll 1
+        for (int x = 0; x < kPer; ++x) {
+          if (x + 1 < kPer) unit(x + 1, w2, at2, sc2, tile2);
+          const int row = at >> 8, c32 = at & 255;
           // the four chunks' order differs between a row's halves so that eight lanes write to eight bank groups
           const int flip = D == 128 ? (c32 >> 1) << 1 : 0;
-          uint32_t w[BITS];
-#pragma unroll
-          for (int i = 0; i < BITS / 4; ++i) *reinterpret_cast<uint4*>(w + 4 * i) = reinterpret_cast<const uint4*>(codes)[i];
-          const T* sc = reinterpret_cast<const T*>(scales);
-          const T* bi = reinterpret_cast<const T*>(scales + kTK * ta.group_bytes);
-          T sv = sc[c32 * 32 >> gs_log], bv = bi[c32 * 32 >> gs_log];
+          T s8 = sc[c32 * 32 >> gs_log], b8 = sc[(c32 * 32 >> gs_log) + kTK * (D >> gs_log)];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             uint32_t w0, w1 = 0;
@@ -1048,10 +1061,12 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
               w1 = flip ? w[2 * (k ^ 2) + 1] : w[2 * k + 1];
             }
             const int c8 = c32 * 4 + (k ^ flip);
-            if (gs_log < 5) sv = sc[c8 * 8 >> gs_log], bv = bi[c8 * 8 >> gs_log];
-            *reinterpret_cast<uint4*>(tile + (c8 >> 3) * kTK * 128 + row * 128 + (((c8 & 7) ^ (row & 7)) << 4)) =
-                dequant8<T, BITS>(w0, w1, sv, bv);
+            if (gs_log < 5) s8 = sc[c8 * 8 >> gs_log], b8 = sc[(c8 * 8 >> gs_log) + kTK * (D >> gs_log)];  // groups inside the unit
+            *reinterpret_cast<uint4*>(tile + (c8 >> 3) * kTK * 128 + (((c8 & 7) ^ (row & 7)) << 4)) = dequant8<T, BITS>(w0, w1, s8, b8);
           }
+#pragma unroll
+          for (int i = 0; i < BITS; ++i) w[i] = w2[i];
+          at = at2, sc = sc2, tile = tile2;
         }
         tc::fence_proxy_async_smem();
         __syncwarp();
@@ -1220,8 +1235,7 @@ struct Plan {
 
 // The tensor-core form takes 16-bit types; packed rows need tiles that start on 16-byte boundaries in the
 // scales too (any capacity that is a multiple of 8 does). The rest runs on the CUDA cores.
-// Units of one length are cut evenly where that uses most of the CTAs that run at once; more parts than
-// √(6·tiles) cost more in the join than they save.
+// Units of one length are cut evenly unless that would leave more than an eighth of the CTAs idle.
 Plan make_plan(int dtype, int bits, int gs, int64_t B, int64_t HKV, int64_t R, int64_t D, int64_t cap, int64_t len_bound,
                bool one_length) {
   Plan p{};
@@ -1236,10 +1250,16 @@ Plan make_plan(int dtype, int bits, int gs, int64_t B, int64_t HKV, int64_t R, i
   p.grid = p.tiles < ctas ? p.tiles : ctas;
   int64_t parts = 2 * p.grid;
   if ((one_length || B == 1) && units <= ctas && B < 65536 && HKV * p.row_tiles < 65536) {
-    int64_t c = ctas / units;
-    if (c > nt) c = nt;
-    while (c > 1 && c * c > 6 * nt) --c;
-    if (c == nt || c < ctas / units || 8 * c * units >= 7 * ctas) {
+    // Parts of a unit: a tile costs about 0.9 us of latency where few are in a part, the join a launch (4 us with
+    // the host's share) and 0.1 us a part.
+    const int64_t most = ctas / units < nt ? ctas / units : nt;
+    int64_t c = 1;
+    double best = 0.9 * nt;
+    for (int64_t k = 2; k <= most; ++k) {
+      const double t = 0.9 * ceil_div(nt, k) + 4.0 + 0.1 * k;
+      if (t < best) best = t, c = k;
+    }
+    if (c < most || most == nt || 8 * c * units >= 7 * ctas) {
       p.cuts = (int)c;
       parts = c * units;
     }
