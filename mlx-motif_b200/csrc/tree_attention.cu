@@ -13,6 +13,7 @@
 // (Line, Schedule), whatever the sequences' lengths: a CTA may end one unit and start the next. A unit
 // that lies in one CTA is normalised and written by it; the others leave fp32 partials (running
 // maximum, Σp, unnormalised O) that tree_merge_kernel joins in a fixed order.
+#include <cooperative_groups.h>
 #include <cuda.h>
 
 #include <cmath>
@@ -45,6 +46,7 @@ struct TreeArgs {
   int B, HKV, gqa, T, R, row_tiles, cap, gs;
   int tile_rows, tile_keys;
   int cuts;                 // > 0: every unit is cut into so many parts, grid (cuts, HKV·row_tiles, B)
+  int cluster;              // the parts of a unit are one thread-block cluster, which joins them itself
   float scale_log2;
 };
 
@@ -60,7 +62,7 @@ __device__ __forceinline__ int key_tiles(const TreeArgs& a, int n) {
 // form one line that is cut into `grid` parts of equal length; where a CTA has many tiles every unit counts
 // `lead` more than it has, since a CTA that ends one unit and begins the next pays for two loads of
 // queries and two outputs.
-constexpr int kLead = 4, kLeadTiles = 8;
+constexpr int kLead = 8, kLeadTiles = 8;
 
 struct Line {
   int total, per, rem, grid, lead;
@@ -136,7 +138,7 @@ struct Schedule {
       at = 1;
       s.b = b, s.g = g, s.rt = rt, s.n = n;
       s.t0 = x0, s.t1 = x1;
-      s.slot = x0 == 0 && x1 == nt ? -1 : (int)((blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x);
+      s.slot = x0 == 0 && x1 == nt && !a.cluster ? -1 : (int)((blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x);
       return true;
     }
     for (;;) {
@@ -246,7 +248,6 @@ __global__ void __launch_bounds__(kSThreads, 2) tree_simt_kernel(const __grid_co
   constexpr int kAcc = kSR * 2 * D / kSThreads;  // rows of one thread in P·V
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int ch = tid % (2 * D), row0 = tid / (2 * D) * kAcc;
-  pdl_trigger();
 
   Schedule sched(a);
   Segment sg;
@@ -392,6 +393,7 @@ struct TcCfg {
 };
 constexpr int kRawMax = 4;
 constexpr int kSBufs = 4;  // S tiles in tensor memory
+constexpr int kMaxCluster = 8;
 
 struct TcArgs {
   TreeArgs t;
@@ -415,7 +417,8 @@ struct TcMap {  // shared memory, bytes from a 1024-byte boundary
   static constexpr int kBar = kV + TcCfg<BITS>::kVStages * kVBytes;
   static constexpr int kNumBars = 1 + 2 * TcCfg<BITS>::kStages + 2 * TcCfg<BITS>::kVStages + 3 * kSBufs + 1 + 2 * kRawMax + 12;
   static constexpr int kState = kBar + kNumBars * 8 + 16;  // [128] reference maxima, [2][128] sums of the groups
-  static constexpr int kBad = kState + 3 * kTR * 4;        // drafted rows cleared: [2 segments][8 warps] Cleared
+  static constexpr int kJoin = kState + 3 * kTR * 4;       // [128] (maximum, sum) of this CTA's part, its rows' weights
+  static constexpr int kBad = kJoin + kTR * 8 + (kTR + 2 * kMaxCluster) * 4;        // drafted rows cleared: [2 segments][8 warps] Cleared
   static constexpr int kRaw = (kBad + 2 * 8 * (int)sizeof(Cleared) + 127) / 128 * 128;
 };
 
@@ -449,6 +452,13 @@ __device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
       : "r"(bar), "r"(parity)
       : "memory");
   return ok != 0;
+}
+
+// Cluster join: channels [4·c4, 4·c4 + 4) of a row of the CTA's unnormalised O, in place of the K and V tiles. Eight rows
+// (lanes that write) and eight chunks of a row (lanes that read) fall into different banks.
+template <int D>
+__device__ __forceinline__ int join_at(int row, int c4) {
+  return row * 2 * D * 4 + ((c4 ^ (row & 7)) << 4);
 }
 
 template <typename T>
@@ -550,7 +560,8 @@ __device__ __forceinline__ uint4 dequant8(uint32_t w0, uint32_t w1, T sc, T bi) 
 // runs for broken inputs only; the finite channels of such an output row are rounded once more per row added.
 template <typename T, int D, int BITS>
 __device__ __forceinline__ void add_cleared(const TreeArgs& a, int b, int g, const Cleared* bad, int seg, int pr, int t,
-                                            int ctx, float m_ref, float inv, int grp, T* yrow, int slot, int row) {
+                                            int ctx, float m_ref, float inv, int grp, T* yrow, int slot, int row,
+                                            uint8_t* joined) {
   const T* q = static_cast<const T*>(a.q) + (((int64_t)b * a.HKV + g) * a.R + pr) * D;
 #pragma unroll 1
   for (int j = 0; j < a.T; ++j) {
@@ -576,12 +587,53 @@ __device__ __forceinline__ void add_cleared(const TreeArgs& a, int b, int g, con
         if (yrow) {
           yrow[c] = from_f<T>(fmaf(p * inv, v[e], to_f<T>(yrow[c])));
         } else {
-          float& o = a.part_o[part_at<D>(a, slot, c >> 3, row) + e];
+          float& o = a.cluster ? reinterpret_cast<float*>(joined + join_at<D>(row, c >> 2))[c & 3]
+                               : a.part_o[part_at<D>(a, slot, c >> 3, row) + e];
           o = fmaf(p, v[e], o);
         }
       }
     }
   }
+}
+
+// The parts of a unit meet in distributed shared memory: CTA `rank` of the cluster joins the rows rank, rank + C, …
+// of all CTAs, O = Σ w·O_s / Σ w·l_s with w = 2^(m_s − max m), in the order of the parts.
+template <typename T, int D>
+__device__ __forceinline__ void join_cluster(const TreeArgs& a, uint8_t* part, float2* ml, float* weights) {
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  cluster.sync();  // every part is in place
+  const int rt = blockIdx.y % a.row_tiles, g = blockIdx.y / a.row_tiles;
+  const int rows = min(kTR, a.R - rt * kTR), mine = rank < rows ? (rows - rank + C - 1) / C : 0;
+  T* y = static_cast<T*>(a.y) + (((int64_t)blockIdx.z * a.HKV + g) * a.R + rt * kTR) * 2 * D;
+  // a row's weights, already over its sum: 16 lanes a row, a lane a part
+  for (int i = threadIdx.x >> 4; i < (mine + 1) / 2 * 2; i += blockDim.x >> 4) {
+    const int s = threadIdx.x & 15;
+    float2 v = make_float2(-INFINITY, 0.f);
+    if (i < mine && s < C) v = *cluster.map_shared_rank(ml + rank + i * C, s);
+    float top = v.x;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float w = v.x == -INFINITY ? 0.f : exp2f(v.x - top), den = v.x == -INFINITY ? v.y : w * v.y;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
+    if (i < mine && s < C) weights[i * C + s] = den == 0.f ? 0.f : den == den ? w / den : NAN;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < mine * (2 * D / 4); i += blockDim.x) {
+    const int k = i / (2 * D / 4), c4 = i % (2 * D / 4), row = rank + k * C;
+    float o[4] = {};
+#pragma unroll 4
+    for (int s = 0; s < C; ++s) {
+      const float w = weights[k * C + s];
+      if (w == 0.f) continue;  // an empty part, or one that saw no key of this row
+      const float4 f = *reinterpret_cast<const float4*>(cluster.map_shared_rank(part, s) + join_at<D>(row, c4));
+      o[0] = fmaf(w, f.x, o[0]), o[1] = fmaf(w, f.y, o[1]), o[2] = fmaf(w, f.z, o[2]), o[3] = fmaf(w, f.w, o[3]);
+    }
+    store_vec<T, 4>(y + (int64_t)row * 2 * D + c4 * 4, o);
+  }
+  cluster.sync();  // the others may still read this CTA's part
 }
 
 template <typename T, int D, int BITS>
@@ -614,7 +666,6 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  pdl_trigger();
   Schedule sched(a);
   Segment sg;
   bool more = sched.next(a, sg);
@@ -658,6 +709,8 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
     for (int i = 0; i < 16; ++i) reinterpret_cast<Cleared*>(smem + Map::kBad)[i].seg = -1;
     tc::mbar_fence_init();
   }
+  float2* join_ml = reinterpret_cast<float2*>(smem + Map::kJoin);
+  if (softmax && grp == 0) join_ml[r] = make_float2(-INFINITY, 0.f);  // a part without a tile
   if (warp == 1) {
     tc::tmem_alloc(tc::smem_addr(tmem_slot), kCols);
     tc::tmem_relinquish();
@@ -729,8 +782,9 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
       // Descriptors as words: the upper ones are one constant (1024-byte atoms, 128-byte swizzle) and the lower
       // ones advance by constants, so that a product costs one addition.
       constexpr uint32_t hi = 1024 >> 4 | 1u << 14 | 2u << 29;
-      const uint32_t q_lo = ((sb + Map::kQ) >> 4) | 1u << 16, k_lo = ((sb + Map::kK) >> 4) | 1u << 16;
-      const uint32_t v_lo = ((sb + Map::kV) >> 4) | (kTK * 128 >> 4) << 16;
+      // in a cluster, shared addresses carry the CTA's rank above the 18 bits that a descriptor holds
+      auto lower = [&](int at, uint32_t lbo) { return ((sb + at) >> 4 & 0x3FFF) | lbo << 16; };
+      const uint32_t q_lo = lower(Map::kQ, 1), k_lo = lower(Map::kK, 1), v_lo = lower(Map::kV, kTK * 128 >> 4);
       auto issue_qk = [&](int j) {
         const int s = j % NS;
         tc::tc_fence_after();
@@ -889,7 +943,7 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
             for (int h = 0; h < Map::kHalves; ++h)
 #pragma unroll 4
               for (int c = 0; c < 8; ++c) {
-                const uint4 v = *reinterpret_cast<const uint4*>(vrow + h * kTK * 128 + c * 16);
+                const uint4 v = *reinterpret_cast<const uint4*>(vrow + h * kTK * 128 + ((c + vr) & 7) * 16);
                 nf |= nonfinite2<T>(v.x) | nonfinite2<T>(v.y) | nonfinite2<T>(v.z) | nonfinite2<T>(v.w);
               }
             clear = nf;
@@ -900,7 +954,7 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
             for (int h = 0; h < Map::kHalves; ++h)
 #pragma unroll 4
               for (int c = 0; c < 8; ++c)
-                *reinterpret_cast<uint4*>(vrow + h * kTK * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(vrow + h * kTK * 128 + ((c + vr) & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
           const bool drafted = clear && pos < sg.n;
           if (__any_sync(0xffffffffu, drafted)) {
@@ -980,7 +1034,8 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
         bool any_bad = false;
 #pragma unroll
         for (int w = 0; w < 8; ++w) any_bad |= bad[w].seg == seg;
-        if (sg.slot >= 0 && live && grp == 0)
+        if (a.cluster && grp == 0) join_ml[r] = make_float2(m_ref, alive ? l : NAN);
+        else if (sg.slot >= 0 && live && grp == 0)
           *reinterpret_cast<float2*>(a.part_ml + ((int64_t)sg.slot * a.slot_rows + r) * 2) = make_float2(m_ref, alive ? l : NAN);
         // a thread writes whole 32-byte sectors of its row
 #pragma unroll 1
@@ -999,6 +1054,11 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
               *reinterpret_cast<uint4*>(dst + 8 * c) =
                   make_uint4(pack2<T>(o[8 * c] * inv, o[8 * c + 1] * inv), pack2<T>(o[8 * c + 2] * inv, o[8 * c + 3] * inv),
                              pack2<T>(o[8 * c + 4] * inv, o[8 * c + 5] * inv), pack2<T>(o[8 * c + 6] * inv, o[8 * c + 7] * inv));
+          } else if (a.cluster) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              *reinterpret_cast<float4*>(smem + Map::kK + join_at<D>(r, cb * 8 + c)) =
+                  make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
           } else {
             float* dst = a.part_o + part_at<D>(a, sg.slot, cb * 4, r);
 #pragma unroll
@@ -1007,7 +1067,7 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
         }
         if (any_bad && alive && live)
           add_cleared<T, D, BITS>(a, sg.b, sg.g, bad, seg, pr, t, ctx, m_ref, inv, grp,
-                                  sg.slot < 0 ? static_cast<T*>(a.y) + row * 2 * D : nullptr, sg.slot, r);
+                                  sg.slot < 0 ? static_cast<T*>(a.y) + row * 2 * D : nullptr, sg.slot, r, smem + Map::kK);
       }
       if (!alive) *abort_flag = 1;
       sg = nx;
@@ -1015,10 +1075,21 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
     }
   } else if constexpr (BITS != 16) {  // ---- operand tiles from packed rows ----
     const int tid = threadIdx.x - 320;
-    const int gs_log = 31 - __clz(a.gs);  // the group size divides 64 or 128
     constexpr int kUnits = kTK * D / 32;  // 32 channels of one row
     constexpr int kFillThreads = Cfg::kThreads - 320, kPer = 3 * kUnits / kFillThreads;
     static_assert(kPer * kFillThreads == 3 * kUnits, "whole units per thread");
+    const int gs_log = 31 - __clz(a.gs);  // the group size divides 64 or 128
+    // A thread's units lie in one 32-channel column, in rows that are equal mod 8: its four chunks' places in a row
+    // are fixed. Their order differs between a row's halves so that eight lanes write to eight bank groups.
+    static_assert(kFillThreads % (8 * (D / 32)) == 0 && kUnits % (8 * (D / 32)) == 0, "one column, one swizzle a thread");
+    const int c32 = tid % (D / 32), flip = D == 128 ? (c32 >> 1) << 1 : 0, bias_at = kTK * (D >> gs_log);
+    const int g_off = (c32 * 32 >> gs_log) * (int)sizeof(T);
+    int off[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int c8 = c32 * 4 + (k ^ flip);
+      off[k] = (c8 >> 3) * kTK * 128 + (((c8 & 7) ^ (tid / (D / 32) & 7)) << 4);
+    }
     int it = 0;
     bool alive = true;
     for (; alive && more; more = sched.next(a, sg)) {
@@ -1029,28 +1100,19 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
                         (it < NS || (bar_wait(k_empty(s), par) && bar_wait(v_empty(s), par)));  // NV is NS here
         if (__any_sync(0xffffffffu, !ok || *abort_flag)) { alive = false; break; }
         const uint8_t* raw = smem + Map::kRaw + rs * (3 * kTK * ta.code_bytes + 6 * kTK * ta.group_bytes);
-        // One short loop (several roles' code shares the instruction caches), the next unit's codes on their way.
-        auto unit = [&](int x, uint32_t (&w)[BITS], int& at, const T*& sc, uint8_t*& tile) {
-          const int u = tid + x * kFillThreads, slot = u / kUnits, row = u % kUnits / (D / 32), c32 = u % (D / 32);
-          const uint4* codes = reinterpret_cast<const uint4*>(raw + (slot * kTK + row) * ta.code_bytes + c32 * BITS * 4);
-#pragma unroll
-          for (int i = 0; i < BITS / 4; ++i) *reinterpret_cast<uint4*>(w + 4 * i) = codes[i];
-          sc = reinterpret_cast<const T*>(raw + 3 * kTK * ta.code_bytes + (slot * 2 * kTK + row) * ta.group_bytes);
-          tile = smem + (slot == 0 ? Map::kK + s * Map::kKBytes : Map::kV + s * Map::kVBytes + (slot - 1) * Map::kKBytes) + row * 128;
-          at = row << 8 | c32;
-        };
-        uint32_t w[BITS], w2[BITS];
-        int at, at2;
-        const T *sc, *sc2;
-        uint8_t *tile, *tile2;
-        unit(0, w, at, sc, tile);
+        uint8_t* kt_ = smem + Map::kK + s * Map::kKBytes;
+        uint8_t* vt_ = smem + Map::kV + s * Map::kVBytes - Map::kKBytes;  // slot 1 and 2: V1, V2
+        const uint8_t* groups = raw + 3 * kTK * ta.code_bytes + g_off;
+        // one short loop: several roles' code shares the instruction caches
 #pragma unroll 1
         for (int x = 0; x < kPer; ++x) {
-          if (x + 1 < kPer) unit(x + 1, w2, at2, sc2, tile2);
-          const int row = at >> 8, c32 = at & 255;
-          // the four chunks' order differs between a row's halves so that eight lanes write to eight bank groups
-          const int flip = D == 128 ? (c32 >> 1) << 1 : 0;
-          T s8 = sc[c32 * 32 >> gs_log], b8 = sc[(c32 * 32 >> gs_log) + kTK * (D >> gs_log)];
+          const int u = tid + x * kFillThreads, slot = u / kUnits, row = u % kUnits / (D / 32);
+          uint32_t w[BITS];
+#pragma unroll
+          for (int i = 0; i < BITS / 4; ++i) *reinterpret_cast<uint4*>(w + 4 * i) = reinterpret_cast<const uint4*>(raw)[u * (BITS / 4) + i];
+          const T* sc = reinterpret_cast<const T*>(groups + (slot * 2 * kTK + row) * ta.group_bytes);
+          uint8_t* tile = (slot == 0 ? kt_ : vt_ + slot * Map::kKBytes) + row * 128;
+          T s8 = sc[0], b8 = sc[bias_at];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             uint32_t w0, w1 = 0;
@@ -1060,13 +1122,9 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
               w0 = flip ? w[2 * (k ^ 2)] : w[2 * k];
               w1 = flip ? w[2 * (k ^ 2) + 1] : w[2 * k + 1];
             }
-            const int c8 = c32 * 4 + (k ^ flip);
-            if (gs_log < 5) s8 = sc[c8 * 8 >> gs_log], b8 = sc[(c8 * 8 >> gs_log) + kTK * (D >> gs_log)];  // groups inside the unit
-            *reinterpret_cast<uint4*>(tile + (c8 >> 3) * kTK * 128 + (((c8 & 7) ^ (row & 7)) << 4)) = dequant8<T, BITS>(w0, w1, s8, b8);
+            if (gs_log < 5) s8 = sc[((k ^ flip) * 8) >> gs_log], b8 = sc[(((k ^ flip) * 8) >> gs_log) + bias_at];  // groups inside the unit
+            *reinterpret_cast<uint4*>(tile + off[k]) = dequant8<T, BITS>(w0, w1, s8, b8);
           }
-#pragma unroll
-          for (int i = 0; i < BITS; ++i) w[i] = w2[i];
-          at = at2, sc = sc2, tile = tile2;
         }
         tc::fence_proxy_async_smem();
         __syncwarp();
@@ -1086,6 +1144,7 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, kCols);
   }
+  if (a.cluster) join_cluster<T, D>(a, smem + Map::kK, join_ml, reinterpret_cast<float*>(join_ml + kTR));
   if (threadIdx.x == 0 && *abort_flag && a.err) atomicExch(a.err, 1);
 }
 
@@ -1137,8 +1196,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps * kMergeRows) tree_merge_kern
     const int from = line.lo(first + k);
     return from >= line.lo(first + k + 1) ? -1 : 2 * (first + k) + (from > at ? 0 : 1);
   };
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");  // every thread: the launch ends after the one before it
-  const bool join = valid && parts > 1;                  // else written by its CTA
+  const bool join = valid && parts > 1;  // else written by its CTA
   const int sub = lane / kChunks, chunk = lane % kChunks;
   float M = -INFINITY, L = 0.f, o[8] = {};
   if (join) {
@@ -1223,11 +1281,20 @@ int sm_count() {  // of the first device asked for: a machine's GPUs are alike
 
 constexpr int64_t kMaxTreeRows = 256;
 
+// Shared memory of the K and V tiles, which a cluster's join takes over.
+int join_room(int bits, int64_t D) {
+  const int k = bits == 16 ? TcMap<128, 16>::kBar - TcMap<128, 16>::kK
+                : bits == 4 ? TcMap<128, 4>::kBar - TcMap<128, 4>::kK
+                            : TcMap<128, 8>::kBar - TcMap<128, 8>::kK;
+  return D == 128 ? k : k / 2;
+}
+
 // Which kernel serves a call, and its launch shape.
 struct Plan {
   bool tc;
   int tile_rows, tile_keys, row_tiles, slot_rows;
   int cuts;       // parts of every unit, or 0: the line
+  bool cluster;   // joined by the cluster of a unit's CTAs, without a second launch
   int64_t tiles;  // key tiles of all units at the longest lengths
   int64_t grid;   // CTAs: at most as many as run at once
   size_t ml_offset, bytes;
@@ -1250,18 +1317,25 @@ Plan make_plan(int dtype, int bits, int gs, int64_t B, int64_t HKV, int64_t R, i
   p.grid = p.tiles < ctas ? p.tiles : ctas;
   int64_t parts = 2 * p.grid;
   if ((one_length || B == 1) && units <= ctas && B < 65536 && HKV * p.row_tiles < 65536) {
-    // Parts of a unit: a tile costs about 0.9 us of latency where few are in a part, the join a launch (4 us with
-    // the host's share) and 0.1 us a part.
+    // Parts of a unit, in us: a tile of a part about 0.9; a join in the cluster 3.5; one by a second launch 5 (with
+    // the host's share) and 0.1 a part. With one CTA an SM only some 64 CTAs run at once as clusters of eight
+    // (16 units of 8 parts took two rounds, 24 us against 14 with a second launch).
     const int64_t most = ctas / units < nt ? ctas / units : nt;
+    const bool room = p.tc && p.slot_rows * 2 * D * 4 <= join_room(bits, D);
     int64_t c = 1;
     double best = 0.9 * nt;
     for (int64_t k = 2; k <= most; ++k) {
-      const double t = 0.9 * ceil_div(nt, k) + 4.0 + 0.1 * k;
+      const double t = 0.9 * ceil_div(nt, k) + 5.0 + 0.1 * k;
       if (t < best) best = t, c = k;
     }
-    if (c < most || most == nt || 8 * c * units >= 7 * ctas) {
+    if (room)
+      for (int64_t k = 2; k <= kMaxCluster && k <= nt && k * units <= 64; ++k) {
+        const double t = 0.9 * ceil_div(nt, k) + 3.5;
+        if (t < best) best = t, c = k, p.cluster = true;
+      }
+    if (p.cluster || c < most || most == nt || 8 * c * units >= 7 * ctas) {
       p.cuts = (int)c;
-      parts = c * units;
+      parts = p.cluster || c == 1 ? 0 : c * units;
     }
   }
   p.ml_offset = sizeof(float) * (size_t)parts * p.slot_rows * 2 * (size_t)D;
@@ -1273,21 +1347,14 @@ dim3 grid_of(const TreeArgs& a, const Plan& p) {
   return a.cuts ? dim3((unsigned)a.cuts, (unsigned)(a.HKV * a.row_tiles), (unsigned)a.B) : dim3((unsigned)p.grid);
 }
 
+// A plain launch: started early (programmatic dependent launch), the join's waiting CTAs cost the attention kernel
+// more than the launch saves (41 against 37 us for a tree of 42 over 16064 rows).
 template <typename T, int D>
 int launch_merge(const TreeArgs& a, const Plan& p, cudaStream_t st) {
-  if (a.cuts == 1) return MOTIF_OK;  // every unit in one part
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)ceil_div((int64_t)a.B * a.HKV * a.R, kMergeRows));
-  cfg.blockDim = dim3(32 * kMergeWarps * kMergeRows);
-  cfg.stream = st;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, tree_merge_kernel<T, D>, a, (int)p.grid);
-  if (e != cudaSuccess) return fail(MOTIF_ERR_CUDA, "sdpa_dual_v_tree: merge launch: %s", cudaGetErrorString(e));
-  return MOTIF_OK;
+  if (a.cuts == 1 || a.cluster) return MOTIF_OK;  // every unit in one part, or joined already
+  const int64_t rows = (int64_t)a.B * a.HKV * a.R;
+  tree_merge_kernel<T, D><<<(unsigned)ceil_div(rows, kMergeRows), 32 * kMergeWarps * kMergeRows, 0, st>>>(a, (int)p.grid);
+  return check_launch("sdpa_dual_v_tree join");
 }
 
 template <typename T, int D, int BITS>
@@ -1324,11 +1391,24 @@ int launch_tc(const TreeArgs& a, const Plan& p, cudaStream_t st) {
     smem += ta.raw_stages * raw;
   }
   auto kern = tree_tc_kernel<T, D, BITS>;
-  static std::atomic<uint64_t> done{0};  // the most that any group size takes
-  const cudaError_t e = once_per_device(
-      done, [&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024); });
-  if (e != cudaSuccess) return fail(MOTIF_ERR_CUDA, "sdpa_dual_v_tree: smem attribute: %s", cudaGetErrorString(e));
-  kern<<<grid_of(a, p), TcCfg<BITS>::kThreads, smem, st>>>(ta);
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = once_per_device(done, [&] {  // the most that any group size takes
+    return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+  });
+  if (e != cudaSuccess) return fail(MOTIF_ERR_CUDA, "sdpa_dual_v_tree: attribute: %s", cudaGetErrorString(e));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid_of(a, p);
+  cfg.blockDim = dim3(TcCfg<BITS>::kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = (unsigned)a.cuts;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = a.cluster ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, kern, ta);
+  if (e != cudaSuccess) return fail(MOTIF_ERR_CUDA, "sdpa_dual_v_tree: %s", cudaGetErrorString(e));
   const int rc = check_launch("sdpa_dual_v_tree");
   return rc ? rc : launch_merge<T, D>(a, p, st);
 }
@@ -1435,9 +1515,10 @@ int motif_sdpa_dual_v_tree(int dtype, int bits, int group_size, const void* q, c
   a.row_tiles = p.row_tiles;
   a.slot_rows = p.slot_rows;
   a.cuts = p.cuts;
+  a.cluster = p.cluster;
   MOTIF_REQUIRE(p.tiles < (1ll << 28), MOTIF_ERR_BAD_SHAPE, "sdpa_dual_v_tree: %lld key tiles in one call",
                 (long long)p.tiles);
-  MOTIF_REQUIRE(workspace && workspace_bytes >= p.bytes, MOTIF_ERR_WORKSPACE,
+  MOTIF_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes), MOTIF_ERR_WORKSPACE,
                 "sdpa_dual_v_tree: workspace of %zu bytes, needs %zu", workspace_bytes, p.bytes);
   MOTIF_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, MOTIF_ERR_BAD_CONTRACT,
                 "sdpa_dual_v_tree: workspace must be 16-byte aligned");

@@ -157,9 +157,9 @@ def _launch(q, parts, strides, bits, group_size, scale, HKV, cap, kv_len, tree_m
         at = [0 if t is None else t.data_ptr() for t in parts]
         kv = motif_tree_kv.from_buffer_copy(_KV.pack(*at[0::3], *at[1::3], *at[2::3], *strides))
         ws_bytes = _workspace_bytes(dev.index, code, bits, group_size, B, HQ, HKV, T, cap, D, cap if n_dev else n, 1 - n_step)
-        ws = workspace(ws_bytes, dev)
+        ws = workspace(ws_bytes, dev) if ws_bytes else None
         check(lib.motif_sdpa_dual_v_tree(code, bits, group_size, qc.data_ptr(), kv, ptr(mask), mask_b, float(scale), B, HQ,
-                                         HKV, T, cap, D, n, n_dev, n_step, y.data_ptr(), ws.data_ptr(), ws_bytes, None,
+                                         HKV, T, cap, D, n, n_dev, n_step, y.data_ptr(), ptr(ws), ws_bytes, None,
                                          stream(dev)), name)
     return y
 

@@ -81,7 +81,8 @@ def test_tree_attention_abi_refusals():
     assert call(cap=1 << 40) == N.ERR_BAD_SHAPE and call(mask=1, mask_b=4) == N.ERR_BAD_SHAPE
     assert call(q=(1 << 20) + 8) == N.ERR_BAD_CONTRACT and b"16-byte" in N.lib.motif_last_error()
     assert call(bits=4, gs=48) == N.ERR_BAD_CONTRACT and call(bits=4, gs=4) == N.ERR_BAD_CONTRACT
-    assert call(wsb=64) == N.ERR_WORKSPACE and call(ws=None) == N.ERR_WORKSPACE
+    long = dict(dtype=2, cap=4096, n=4096)  # parts that meet in the workspace
+    assert call(wsb=64, **long) == N.ERR_WORKSPACE and call(ws=None, **long) == N.ERR_WORKSPACE
     kv.stride[2] = 130
     assert call() == N.ERR_BAD_CONTRACT and b"strides" in N.lib.motif_last_error()
     kv.stride[2] = 128
