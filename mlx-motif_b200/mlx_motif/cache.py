@@ -22,6 +22,8 @@ form a captured CUDA graph needs.
 
 from __future__ import annotations
 
+import struct
+
 import torch
 
 from ._native import check, dtype_code, lib, motif_kv4_slots, on_device, ptr, stream
@@ -46,24 +48,12 @@ def create_attention_mask(N: int, offset: int = 0, return_array: bool = False, w
     return "causal"
 
 
+_SLOTS = struct.Struct("12q2i4q")  # motif_kv4_slots: data, scales, biases of the four slots, then the sizes
+
+
 def _slots_struct(slots, bits: int, group_size: int, B: int, H: int, cap: int, D: int) -> motif_kv4_slots:
-    s = motif_kv4_slots()
-    for i, slot in enumerate(slots):
-        if bits == 16:
-            s.data[i] = ptr(slot)
-            s.scales[i] = None
-            s.biases[i] = None
-        else:
-            s.data[i] = ptr(slot[0])
-            s.scales[i] = ptr(slot[1])
-            s.biases[i] = ptr(slot[2])
-    s.bits = bits
-    s.group_size = group_size
-    s.batch = B
-    s.heads = H
-    s.capacity = cap
-    s.head_dim = D
-    return s
+    at = [ptr(t) or 0 for t in slots] + [0] * 8 if bits == 16 else [ptr(slot[i]) for i in range(3) for slot in slots]
+    return motif_kv4_slots.from_buffer_copy(_SLOTS.pack(*at, bits, group_size, B, H, cap, D))
 
 
 def _filled(slots) -> list:
@@ -82,13 +72,13 @@ class KVSlots:
             raise ValueError("kv_slots: no caches")
         self.buffers = [c._buffers() for c in caches]
         first = self.buffers[0][-1]  # a row or scale buffer: its type and device are the cache's
+        self.device, dtype = first.device, first.dtype
         for bufs in self.buffers:
             for t in bufs:
-                if t.device != first.device:
-                    raise ValueError(f"caches on {t.device} and {first.device}: all must be on one CUDA device")
-            if bufs[-1].dtype != first.dtype:
-                raise TypeError(f"caches of {bufs[-1].dtype} and {first.dtype}: all must have one type")
-        self.device = first.device
+                if t.device != self.device:
+                    raise ValueError(f"caches on {t.device} and {self.device}: all must be on one CUDA device")
+            if bufs[-1].dtype != dtype:
+                raise TypeError(f"caches of {bufs[-1].dtype} and {dtype}: all must have one type")
         self.dtype_code = dtype_code(first)
         self.structs = (motif_kv4_slots * len(caches))(*(c.slots_struct() for c in caches))
         s = self.structs[0]
@@ -120,7 +110,7 @@ def keep_rows(slots: KVSlots, path: torch.Tensor, accepted: torch.Tensor, base) 
         if t.device != dev:
             raise ValueError(f"{name} on {t.device}, the caches on {dev}")
     assert path.dim() == 2 and path.shape[0] == B, f"path {tuple(path.shape)} must be ({B}, T)"
-    assert tuple(accepted.shape) == (B,), f"accepted {tuple(accepted.shape)} must be ({B},)"
+    assert accepted.shape == (B,), f"accepted {tuple(accepted.shape)} must be ({B},)"
     T = path.shape[1]
     base_dev, base_step, base_host = None, 0, 0
     if isinstance(base, torch.Tensor):

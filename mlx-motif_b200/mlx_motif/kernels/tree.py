@@ -123,7 +123,7 @@ def _check_mask(mask, B: int, T: int, device):
         return None, 0
     if mask.dtype != torch.bool:
         raise TypeError(f"tree_mask must be a bool tensor, got {mask.dtype}")
-    assert tuple(mask.shape) in ((T, T), (B, T, T)), f"tree_mask {tuple(mask.shape)} must be ({T}, {T}) or ({B}, {T}, {T})"
+    assert mask.shape == (T, T) or mask.shape == (B, T, T), f"tree_mask {tuple(mask.shape)} must be ({T}, {T}) or ({B}, {T}, {T})"
     _check_device(mask, device)
     return contiguous(mask), T * T if mask.dim() == 3 else 0
 
@@ -148,7 +148,7 @@ def _launch(q, parts, strides, bits, group_size, scale, HKV, cap, kv_len, tree_m
             _check_device(t, dev)
     n, n_dev, n_step = _check_len(kv_len, B, T, cap, dev)
     mask, mask_b = _check_mask(tree_mask, B, T, dev)
-    y = torch.empty((B, HQ, T, 2 * D), dtype=q.dtype, device=dev)
+    y = q.new_empty((B, HQ, T, 2 * D))
     if B == 0 or cap == 0:
         return y.zero_()
     with on_device(dev):
@@ -184,10 +184,14 @@ def sdpa_dual_v_tree(q: torch.Tensor, k: torch.Tensor, v1: torch.Tensor, v2: tor
     assert k.shape == v1.shape == v2.shape == (B, HKV, cap, D), "k, v1, v2 must match (B, H_kv, KV_cap, D)"
     if not k.dtype == v1.dtype == v2.dtype == q.dtype:
         k, v1, v2 = (t.to(q.dtype) for t in (k, v1, v2))
-    strides = _row_strides(k)
-    if strides is None or _row_strides(v1) != strides or _row_strides(v2) != strides:
-        k, v1, v2 = (_aligned(t) for t in (k, v1, v2))
-        strides = _row_strides(k) if cap else (0, 0, 0)
+    if k.is_contiguous() and v1.is_contiguous() and v2.is_contiguous() and \
+            (k.data_ptr() | v1.data_ptr() | v2.data_ptr()) % 16 == 0:
+        strides = (HKV * cap * D, cap * D, D)
+    else:
+        strides = _row_strides(k)
+        if strides is None or _row_strides(v1) != strides or _row_strides(v2) != strides:
+            k, v1, v2 = (_aligned(t) for t in (k, v1, v2))
+            strides = (HKV * cap * D, cap * D, D)
     return _launch(q, (k, None, None, v1, None, None, v2, None, None), strides, 16, 64, scale, HKV, cap, kv_len, tree_mask,
                    "sdpa_dual_v_tree")
 

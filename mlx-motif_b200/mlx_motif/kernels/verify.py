@@ -118,13 +118,12 @@ def speculative_verify(tokens: torch.Tensor, parents: torch.Tensor, p_logits: to
     assert p_logits.dim() == 3, f"p_logits {tuple(p_logits.shape)} must be (B, T, V)"
     B, T, V = p_logits.shape
     assert T >= 1 and V >= 1, f"p_logits {tuple(p_logits.shape)} must have a row and a token"
-    assert tuple(tokens.shape) == (B, T), f"tokens {tuple(tokens.shape)} must be ({B}, {T})"
-    assert tuple(parents.shape) in ((T,), (B, T)), f"parents {tuple(parents.shape)} must be ({T},) or ({B}, {T})"
+    assert tokens.shape == (B, T), f"tokens {tuple(tokens.shape)} must be ({B}, {T})"
+    assert parents.shape == (B, T) or parents.shape == (T,), f"parents {tuple(parents.shape)} must be ({T},) or ({B}, {T})"
     assert math.isfinite(temperature) and temperature >= 0, f"temperature {temperature} must be finite and >= 0"
     dev = p_logits.device
-    for t, name in ((tokens, "tokens"), (parents, "parents")):
-        if t.dtype != torch.int32:
-            raise TypeError(f"{name} must be int32, got {t.dtype}")
+    if tokens.dtype != torch.int32 or parents.dtype != torch.int32:
+        raise TypeError(f"tokens and parents must be int32, got {tokens.dtype} and {parents.dtype}")
     code = dtype_code(p_logits)
     sampled = temperature > 0
     R = 0
@@ -132,17 +131,16 @@ def speculative_verify(tokens: torch.Tensor, parents: torch.Tensor, p_logits: to
         assert q_logits is not None and uniforms is not None, "q_logits and uniforms are needed at a temperature > 0"
         assert q_logits.dim() == 3 and q_logits.shape[0] == B and q_logits.shape[2] == V and 1 <= q_logits.shape[1] <= T, \
             f"q_logits {tuple(q_logits.shape)} must be ({B}, 1..{T}, {V})"
-        assert tuple(uniforms.shape) == (B, T), f"uniforms {tuple(uniforms.shape)} must be ({B}, {T})"
+        assert uniforms.shape == (B, T), f"uniforms {tuple(uniforms.shape)} must be ({B}, {T})"
         if q_logits.dtype != p_logits.dtype:
             raise TypeError(f"q_logits {q_logits.dtype} and p_logits {p_logits.dtype} must have one type")
         if uniforms.dtype != torch.float32:
             raise TypeError(f"uniforms must be float32, got {uniforms.dtype}")
         R = q_logits.shape[1]
-    for t in (tokens, parents) + ((q_logits, uniforms) if sampled else ()):
+    for t in (tokens, parents, q_logits, uniforms) if sampled else (tokens, parents):
         if t.device != dev:
             raise ValueError(f"tensors on {t.device} and {dev}: all operands must be on one CUDA device")
-    both = torch.empty((2, B), dtype=torch.int32, device=dev)  # one allocation for the counts and the tokens
-    out = VerifyResult(both[0], torch.empty((B, T), dtype=torch.int32, device=dev), both[1])
+    out = VerifyResult(tokens.new_empty(B), tokens.new_empty((B, T)), tokens.new_empty(B))
     if B == 0:
         return out
     with on_device(dev):
@@ -152,10 +150,11 @@ def speculative_verify(tokens: torch.Tensor, parents: torch.Tensor, p_logits: to
         u = contiguous(uniforms) if sampled else None
         ws_bytes = _workspace_bytes(B, T, R, V)
         ws = workspace(ws_bytes, dev)
+        accepted, path, next_token = out
         pb, pr, _ = p.stride()
         qb, qr, _ = q.stride() if sampled else (0, 0, 0)
         check(lib.motif_speculative_verify(code, p.data_ptr(), pb, pr, ptr(q), qb, qr, R, tok.data_ptr(), par.data_ptr(),
                                            T if parents.dim() == 2 else 0, ptr(u), B, T, V, temperature,
-                                           out.accepted.data_ptr(), out.path.data_ptr(), out.next_token.data_ptr(),
+                                           accepted.data_ptr(), path.data_ptr(), next_token.data_ptr(),
                                            ws.data_ptr(), ws_bytes, stream(dev)), "speculative_verify")
     return out
