@@ -106,9 +106,23 @@ __device__ __forceinline__ unsigned long long warp_max_u64(unsigned long long v)
   return v;
 }
 
+// Larger of two packed pairs; a NaN loses.
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b, __half) {
+  const __half2 m = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b, __nv_bfloat16) {
+  const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b, float) {
+  return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+}
+
 // One chunk of one row: [lo, hi), lo on a 16-byte boundary of the row but for the first chunk, whose few entries
-// before the boundary are its `head`.
-template <typename T>
+// before the boundary are its `head`. Issue-bound before the pairs' maxima and the plain sum were taken apart from
+// the rare cases (13.7 instructions an entry: 17 us for 127 rows of 219520; now about 6).
+template <typename T, bool GREEDY>
 __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(VerifyArgs a) {
   constexpr int kVec = 16 / (int)sizeof(T), kLoads = kChunk / kVec / kStatThreads;
   __shared__ float sf[8];
@@ -120,11 +134,13 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(VerifyArgs a
   const int shift = min((int)((16 - reinterpret_cast<uintptr_t>(l) % 16) % 16 / sizeof(T)), a.V);
   const int lo = min(c * kChunk + shift, a.V), hi = c + 1 == a.chunks ? a.V : min(lo + kChunk, a.V);
   const int n_vec = (hi - lo) / kVec;
+  // a place without a vector holds -inf throughout
+  const uint32_t none = sizeof(T) == 4 ? 0xFF800000u : std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
   uint4 raw[kLoads];
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
     const int v = tid + i * kStatThreads;
-    if (v < n_vec) raw[i] = reinterpret_cast<const uint4*>(l + lo)[v];
+    raw[i] = v < n_vec ? reinterpret_cast<const uint4*>(l + lo)[v] : make_uint4(none, none, none, none);
   }
   // the entries outside whole vectors: before the first chunk's boundary, and behind the last vector
   const int tail0 = lo + n_vec * kVec;
@@ -132,25 +148,19 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(VerifyArgs a
   if (c == 0 && tid < shift) edge = tid;
   if (tid >= 32 && tail0 + tid - 32 < hi) edge = tail0 + tid - 32;
   const float ev = edge >= 0 ? logit(l, edge) : -INFINITY;
-  float m = ev;
-  unsigned long long top = edge >= 0 ? top_key(ev, edge) : 0;
-  const bool greedy = a.inv_t == 0.0;
+  if constexpr (GREEDY) {
+    unsigned long long top = edge >= 0 ? top_key(ev, edge) : 0;
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int v = tid + i * kStatThreads;
-    if (v >= n_vec) continue;
-    const T* e = reinterpret_cast<const T*>(&raw[i]);
+    for (int i = 0; i < kLoads; ++i) {
+      const int v = tid + i * kStatThreads;
+      if (v >= n_vec) continue;
+      const T* e = reinterpret_cast<const T*>(&raw[i]);
 #pragma unroll
-    for (int x = 0; x < kVec; ++x) {
-      const float f = logit(e, x);
-      m = fmaxf(m, f);
-      if (greedy) {
-        const unsigned long long k = top_key(f, lo + v * kVec + x);
+      for (int x = 0; x < kVec; ++x) {
+        const unsigned long long k = top_key(logit(e, x), lo + v * kVec + x);
         top = k > top ? k : top;
       }
     }
-  }
-  if (greedy) {
     top = warp_max_u64(top);
     if (lane == 0) sk[warp] = top;
     __syncthreads();
@@ -161,6 +171,13 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(VerifyArgs a
     }
     return;
   }
+  uint32_t mx = none;
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i)
+    mx = max2(mx, max2(max2(raw[i].x, raw[i].y, T{}), max2(raw[i].z, raw[i].w, T{}), T{}), T{});
+  const T* pair = reinterpret_cast<const T*>(&mx);
+  float m = fmaxf(ev, logit(pair, 0));
+  if (sizeof(T) == 2) m = fmaxf(m, logit(pair, sizeof(T) == 2 ? 1 : 0));
   m = warp_max(m);
   if (lane == 0) sf[warp] = m;
   __syncthreads();
@@ -168,27 +185,26 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(VerifyArgs a
   for (int w = 0; w < 8; ++w) m = fmaxf(m, sf[w]);
   const float k = (float)a.inv_t * 1.4426950408889634f;
   float z = 0.f;
-  if (m == INFINITY) {  // the infinite entries share the law
-    z = ev == m ? 1.f : 0.f;
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int v = tid + i * kStatThreads;
-      if (v >= n_vec) continue;
-      const T* e = reinterpret_cast<const T*>(&raw[i]);
-#pragma unroll
-      for (int x = 0; x < kVec; ++x) z += to_f<T>(e[x]) == m ? 1.f : 0.f;
-    }
-  } else if (m > -INFINITY) {
+  if (fabsf(m) < INFINITY) {
     float zs[4] = {edge >= 0 ? ex2((ev - m) * k) : 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int v = tid + i * kStatThreads;
-      if (v >= n_vec) continue;
       const T* e = reinterpret_cast<const T*>(&raw[i]);
 #pragma unroll
-      for (int x = 0; x < kVec; ++x) zs[x & 3] += ex2((logit(e, x) - m) * k);
+      for (int x = 0; x < kVec; ++x) zs[x & 3] += ex2((to_f<T>(e[x]) - m) * k);
     }
     z = (zs[0] + zs[1]) + (zs[2] + zs[3]);
+  }
+  if (m == INFINITY || z != z) {  // infinite entries share the law; a NaN counts as -inf
+    auto term = [&](float f) { return m == INFINITY ? (f == m ? 1.f : 0.f) : ex2((f - m) * k); };
+    z = edge >= 0 ? term(ev) : 0.f;
+#pragma unroll 1
+    for (int i = 0; i < kLoads; ++i) {
+      const int v = tid + i * kStatThreads;
+      if (v >= n_vec) break;
+#pragma unroll 1
+      for (int x = 0; x < kVec; ++x) z += term(logit(l, lo + v * kVec + x));
+    }
   }
   z = warp_sum(z);
   __syncthreads();
@@ -254,17 +270,21 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyArgs a)
   }
   if (!greedy && tid < kTable) table[tid] = exp2(tid / (double)kTable);
   __syncthreads();
-  for (int i = tid; i < a.T; i += kWalkThreads) {
-    int f = -1, n = -1;
-    const int mine = par[i];
+  // links: a warp finds a row's children, 32 rows a ballot, from the last to the first
 #pragma unroll 1
-    for (int j = a.T - 1; j > i; --j) {
-      const int pj = par[j];
-      f = pj == i ? j : f;
-      n = pj == mine ? j : n;
+  for (int i = warp; i < a.T; i += kWalkWarps) {
+    int after = -1;  // the child that follows those of this ballot
+#pragma unroll 1
+    for (int j0 = (a.T - 1) & ~31; j0 + 31 > i; j0 -= 32) {
+      const int j = j0 + lane;
+      const bool mine = j < a.T && par[j] == i;
+      const unsigned kids = __ballot_sync(0xffffffffu, mine);
+      const unsigned later = lane < 31 ? kids >> (lane + 1) : 0;
+      if (mine) next[j] = later ? j + __ffs(later) : after;
+      after = kids ? j0 + __ffs(kids) - 1 : after;
+      if (j0 == 0) break;
     }
-    first[i] = f;
-    next[i] = n;
+    if (lane == 0) first[i] = after;
   }
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
   // the rows' laws (τ = 0: their largest entries) from the chunks: eight lanes a row
@@ -536,7 +556,9 @@ int chunks_of(int64_t V) { return (int)ceil_div(V, kChunk); }
 template <typename T>
 int launch_verify(const VerifyArgs& a, int64_t batch, cudaStream_t st) {
   const bool greedy = a.inv_t == 0.0;
-  verify_stats_kernel<T><<<dim3((unsigned)a.chunks, (unsigned)(a.T + (greedy ? 0 : a.R)), (unsigned)batch), kStatThreads, 0, st>>>(a);
+  const dim3 chunks((unsigned)a.chunks, (unsigned)(a.T + a.R), (unsigned)batch);
+  if (greedy) verify_stats_kernel<T, true><<<chunks, kStatThreads, 0, st>>>(a);
+  else verify_stats_kernel<T, false><<<chunks, kStatThreads, 0, st>>>(a);
   const int rc = check_launch("speculative_verify");
   if (rc) return rc;
   // CTAs of a cluster: all SMs together serve the batch, and a CTA has 2048 entries or more
