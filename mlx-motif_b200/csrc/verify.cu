@@ -632,11 +632,11 @@ int motif_speculative_verify(int dtype, const void* p_logits, int64_t p_batch_st
                              size_t workspace_bytes, void* stream) {
   MOTIF_REQUIRE(p_logits && tokens && parents && accepted && path && next_token, MOTIF_ERR_NULL,
                 "speculative_verify: null pointer");
-  MOTIF_REQUIRE(std::isfinite(temperature) && temperature >= 0.0, MOTIF_ERR_BAD_CONTRACT,
-                "speculative_verify: temperature %f", temperature);
+  MOTIF_REQUIRE(temperature == 0.0 || (temperature >= 1e-6 && temperature <= 1e6), MOTIF_ERR_BAD_CONTRACT,
+                "speculative_verify: temperature %g (0, or 1e-6 .. 1e6)", temperature);
   MOTIF_REQUIRE(temperature == 0.0 || (q_logits && uniforms), MOTIF_ERR_NULL,
                 "speculative_verify: q_logits and uniforms are needed at temperature %f", temperature);
-  MOTIF_REQUIRE(batch >= 1 && batch < 65536 && rows >= 1 && rows <= kMaxRows && vocab >= 1 && vocab < (1ll << 31),
+  MOTIF_REQUIRE(batch >= 1 && batch < 65536 && rows >= 1 && rows <= kMaxRows && vocab >= 1 && vocab < (1ll << 30),
                 MOTIF_ERR_BAD_SHAPE, "speculative_verify: batch=%lld rows=%lld (1..1024) vocab=%lld", (long long)batch,
                 (long long)rows, (long long)vocab);
   MOTIF_REQUIRE(temperature == 0.0 || (draft_rows >= 1 && draft_rows <= rows), MOTIF_ERR_BAD_SHAPE,

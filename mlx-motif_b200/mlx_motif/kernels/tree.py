@@ -98,7 +98,7 @@ def _check_q(q, shape_kv, name: str):
     B, HQ, T, D = q.shape
     HKV, cap = shape_kv[1], shape_kv[2]
     assert D % 32 == 0, f"D={D} must be a multiple of 32"
-    assert HQ % HKV == 0, f"H_q={HQ} must be a multiple of H_kv={HKV}"
+    assert HKV >= 1 and HQ >= 1 and HQ % HKV == 0, f"H_q={HQ} must be a multiple of H_kv={HKV}"
     assert 1 <= T <= MAX_TREE_ROWS, f"{name} takes 1..{MAX_TREE_ROWS} tree rows, got {T}"
     return B, HQ, T, D, HKV, cap
 

@@ -110,7 +110,8 @@ def speculative_verify(tokens: torch.Tensor, parents: torch.Tensor, p_logits: to
     from the last w. At ``temperature`` 0 (q_logits and uniforms may be None) a child is accepted if it is the
     target's argmax. Returns (accepted, path, next_token) on the device: no synchronisation.
 
-    A token outside [0, V) is never accepted (padding of a smaller tree). NaN logits count as −inf.
+    A token outside [0, V) is never accepted (padding of a smaller tree). NaN logits count as −inf. ``temperature``
+    is 0 or in [1e-6, 1e6].
     """
     if _DISABLE:
         return speculative_verify_reference(tokens, parents, p_logits, q_logits, uniforms, temperature)
@@ -120,7 +121,7 @@ def speculative_verify(tokens: torch.Tensor, parents: torch.Tensor, p_logits: to
     assert T >= 1 and V >= 1, f"p_logits {tuple(p_logits.shape)} must have a row and a token"
     assert tokens.shape == (B, T), f"tokens {tuple(tokens.shape)} must be ({B}, {T})"
     assert parents.shape == (B, T) or parents.shape == (T,), f"parents {tuple(parents.shape)} must be ({T},) or ({B}, {T})"
-    assert math.isfinite(temperature) and temperature >= 0, f"temperature {temperature} must be finite and >= 0"
+    assert temperature == 0 or 1e-6 <= temperature <= 1e6, f"temperature {temperature} must be 0 or in [1e-6, 1e6]"
     dev = p_logits.device
     if tokens.dtype != torch.int32 or parents.dtype != torch.int32:
         raise TypeError(f"tokens and parents must be int32, got {tokens.dtype} and {parents.dtype}")

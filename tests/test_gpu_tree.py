@@ -177,6 +177,41 @@ def test_tree_attention(cuda, B, HQ, HKV, T, D, cap, n, mask, dtype, bits, gs):
     assert torch.equal(got, call(q, kv, bits, gs, scale, kv_len=n, tree_mask=m))  # a fixed order of sums
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("bits,gs,D", [(4, 8, 128), (4, 16, 128), (4, 128, 128), (4, 8, 64), (8, 8, 128), (8, 16, 64),
+                                       (8, 128, 128)])
+def test_tree_attention_group_sizes(cuda, dtype, bits, gs, D):
+    """Groups within a chunk of eight channels up to a whole row, in tiles that several parts share."""
+    B, HQ, HKV, T, cap, n = 2, 6, 2, 11, 1024, 901
+    g = torch.Generator(device="cuda").manual_seed(gs)
+    q = torch.randn((B, HQ, T, D), generator=g, device="cuda").to(DT[dtype])
+    packed = []
+    for _ in range(3):
+        words = torch.randint(-(2**31), 2**31, (B, HKV, cap, D * bits // 32), generator=g, device="cuda").int().view(torch.uint32)
+        scales = (torch.rand((B, HKV, cap, D // gs), generator=g, device="cuda") * 2.0 / 2**bits + 0.01).to(DT[dtype])
+        biases = (torch.randn((B, HKV, cap, D // gs), generator=g, device="cuda") * 0.5 - 1.0).to(DT[dtype])
+        packed.append((words, scales, biases))
+    m, m64 = masks("trees", B, T)
+    got = call(q, packed, bits, gs, 0.05, kv_len=n, tree_mask=m)
+    want, tol = attention64(q, *(unpack64(t, bits, gs) for t in packed), 0.05, [n] * B, m64, torch.finfo(DT[dtype]).eps / 2, True)
+    check(got, want, tol, dtype)
+
+
+@pytest.mark.parametrize("dtype,bits", [("fp16", 16), ("bf16", 4), ("fp16", 8), ("fp32", 16)])
+@pytest.mark.parametrize("cap", [640, 16384])
+def test_tree_attention_one_device_length(cuda, dtype, bits, cap):
+    """One length on the device, the launch shaped for the capacity: parts without a tile, an empty cache."""
+    B, HQ, HKV, T, D = 1, 6, 2, 9, 128
+    q, kv, plain = make(2, B, HQ, HKV, T, D, cap, dtype, bits)
+    m, m64 = masks("trees", B, T)
+    n_dev = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for n in (0, 3, 9, 64, 65, 200, 640):
+        n_dev.fill_(n)
+        got = call(q, kv, bits, 64, 0.1, kv_len=n_dev, tree_mask=m)
+        want, tol = attention64(q, *plain, 0.1, [n], m64, torch.finfo(DT[dtype]).eps / 2, bits != 16)
+        check(got, want, tol, dtype, str(n))
+
+
 @pytest.mark.parametrize("dtype,bits", [("fp16", 16), ("fp32", 16), ("bf16", 4)])
 def test_tree_attention_device_lengths(cuda, dtype, bits):
     """One length per sequence read on the device: empty, shorter than the tree, beyond the capacity."""
@@ -196,10 +231,11 @@ def test_tree_attention_device_lengths(cuda, dtype, bits):
 
 @pytest.mark.parametrize("dtype,bits", [("fp16", 16), ("bf16", 16), ("fp32", 16), ("fp16", 4)])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
-def test_tree_attention_hidden_rows_may_hold_anything(cuda, dtype, bits, bad):
+@pytest.mark.parametrize("n", [190, 700, 9000])  # a unit in one CTA, in a cluster, in parts joined by a second launch
+def test_tree_attention_hidden_rows_may_hold_anything(cuda, dtype, bits, bad, n):
     """Rows behind the last live one, and drafted rows as seen by queries they are hidden from, do not reach
     a result; queries that see such a row get what the formula gives."""
-    B, HQ, HKV, T, D, cap, n = 1, 4, 2, 6, 128, 256, 190
+    B, HQ, HKV, T, D, cap = 1, 4, 2, 6, 128, 9216
     q, kv, plain = make(3, B, HQ, HKV, T, D, cap, dtype, bits)
     par = [-1, 0, 0, 1, 1, 2]
     m = ancestors(par)

@@ -23,6 +23,8 @@ def test_tree_attention_refusals():
         sdpa_dual_v_tree(torch.zeros(1, 4, 3, 40), *(torch.zeros(1, 2, 16, 40) for _ in range(3)), 0.1)
     with pytest.raises(AssertionError, match="multiple of H_kv"):
         sdpa_dual_v_tree(q[:, :3], *kv, 0.1)
+    with pytest.raises(AssertionError, match="multiple of H_kv"):
+        sdpa_dual_v_tree(q, *(t[:, :0] for t in kv), 0.1)
     with pytest.raises(AssertionError, match="must match"):
         sdpa_dual_v_tree(q, kv[0], kv[1][:, :, :8], kv[2], 0.1)
     with pytest.raises(AssertionError, match="1..256 tree rows"):
@@ -110,7 +112,7 @@ def test_verify_refusals():
         speculative_verify(tok, par, p, None, u, 1.0)
     with pytest.raises(AssertionError, match="uniforms"):
         speculative_verify(tok, par, p, q, u[:, :2], 1.0)
-    for bad in (-0.5, float("nan"), float("inf")):
+    for bad in (-0.5, float("nan"), float("inf"), 1e-9, 1e9):
         with pytest.raises(AssertionError, match="temperature"):
             speculative_verify(tok, par, p, q, u, bad)
     with pytest.raises(TypeError, match="int32"):
@@ -134,6 +136,7 @@ def test_verify_abi_refusals():
 
     assert call(p=None) == N.ERR_NULL and call(q=None) == N.ERR_NULL and call(u=None) == N.ERR_NULL
     assert call(out=None) == N.ERR_NULL
+    assert call(V=1 << 30) == N.ERR_BAD_SHAPE and call(temp=1e-7) == N.ERR_BAD_CONTRACT
     assert call(temp=-1.0) == N.ERR_BAD_CONTRACT and call(temp=float("nan")) == N.ERR_BAD_CONTRACT
     assert call(R=3) == N.ERR_BAD_SHAPE and call(T=0) == N.ERR_BAD_SHAPE and call(T=1025) == N.ERR_BAD_SHAPE
     assert call(V=0) == N.ERR_BAD_SHAPE and call(par_b=1) == N.ERR_BAD_SHAPE
