@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(kSThreads, 2) tree_simt_kernel(const __grid_co
 //   warp 0       TMA: K and V tiles straight from the cache into rings of kStages (16-bit rows), or the
 //                packed rows, scales and biases into a ring of raw tiles;
 //   warp 1       one lane issues the MMAs, S up to kSBufs tiles ahead of P·V within a segment, so that the
-//                softmax groups find their tiles ready;
+//                softmax groups find their tiles ready (16-bit rows: S from warp 1, P·V from warp 10);
 //   warps 2..9   two softmax groups of four warps that take the tiles in turn (one warp alone on a
 //                scheduler waits out every latency of its 64-column row: tensor-memory reads, the maximum,
 //                the exponentials). A thread is a query row: it takes S from tensor memory and writes P in
@@ -388,7 +388,7 @@ struct TcCfg {
   // (8-bit ones are twice as large).
   static constexpr int kStages = BITS == 8 ? 2 : 3;
   static constexpr int kVStages = BITS == 16 ? 4 : BITS == 4 ? 3 : 2;
-  static constexpr int kThreads = BITS == 16 ? 320 : 512;
+  static constexpr int kThreads = BITS == 16 ? 352 : 512;
   static constexpr int kFill = BITS == 16 ? 1 : 6;  // arrivals that fill a K or V tile
 };
 constexpr int kRawMax = 4;
@@ -703,6 +703,7 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
       if (i >= kB2 && i < kB2 + kSBufs) count = 4;                                            // p_full
       if (i >= kB3 + kRawMax && i < kB4) count = Cfg::kFill;                                  // raw_empty
       if (i >= kB4 + 8) count = 2;                                                            // l_both
+      if (i == kB2 + 2 * kSBufs) count = BITS == 16 ? 2 : 1;                                  // drain
       tc::mbar_init(bar + 8u * i, count);
     }
     *abort_flag = 0;
@@ -775,7 +776,7 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
       for (int j = max(0, v_iss - NV); j < v_iss; ++j)
         if (!bar_wait(v_full(j % NV), (j / NV) & 1)) *abort_flag = 1;
     }
-  } else if (warp == 1) {
+  } else if (warp == 1 || (BITS == 16 && warp == 10)) {
     if (lane == 0) {  // ---- MMAs ----
       constexpr uint32_t idesc_qk = tc::idesc_f16_f32(kTR, kTK, false, false, kBf16);
       constexpr uint32_t idesc_pv = tc::idesc_f16_f32(kTR, 2 * D, true, false, kBf16);
@@ -805,25 +806,44 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
         tc::mma_commit(o_done(j % kSBufs));
         tc::mma_commit(v_empty(j % NV));
       };
-      int it = 0, qn = 0, seg = 0;  // the next P·V, the next S
       bool ok = true;
-      for (; ok && more; more = sched.next(a, sg), ++seg) {
-        ok = bar_wait(q_full, seg & 1);
-        const int end = it + sg.t1 - sg.t0, begin = it;
-        // S runs up to kSBufs tiles ahead of P·V; its buffer is free once the P·V of kSBufs tiles before has read P there.
-        for (int polls = 0; ok && it < end;) {
-          const bool s_ahead = qn < end && qn < it + kSBufs &&
-                               (qn < kSBufs || bar_test(o_done(qn % kSBufs), (qn / kSBufs - 1) & 1));
-          if (s_ahead && (qn <= it + 1 || !bar_test(p_full(it % kSBufs), (it / kSBufs) & 1)) &&
-              bar_test(k_full(qn % NS), (qn / NS) & 1)) {
-            issue_qk(qn++);
-            polls = 0;
-          } else if (qn > it && bar_test(p_full(it % kSBufs), (it / kSBufs) & 1) && bar_test(v_full(it % NV), (it / NV) & 1)) {
-            issue_pv(it, it > begin);
-            ++it;
-            polls = 0;
-          } else if (++polls > kTestPolls || *abort_flag) {
-            ok = false;
+      if constexpr (BITS == 16) {
+        // Two issuers: products of one thread wait for its own polls and issue slots (0.36 us an S, 0.19 us a P·V and
+        // as much again between them: 1.15 us a tile from one thread).
+        int it = 0, seg = 0;
+        for (; ok && more; more = sched.next(a, sg), ++seg) {
+          if (warp == 1) ok = bar_wait(q_full, seg & 1);
+          for (int kt = sg.t0; ok && kt < sg.t1; ++kt, ++it) {
+            if (warp == 1) {  // S: its buffer is free once the P·V of kSBufs tiles before has read P there
+              ok = (it < kSBufs || bar_wait(o_done(it % kSBufs), (it / kSBufs - 1) & 1)) && bar_wait(k_full(it % NS), (it / NS) & 1);
+              if (ok) issue_qk(it);
+            } else {
+              ok = bar_wait(p_full(it % kSBufs), (it / kSBufs) & 1) && bar_wait(v_full(it % NV), (it / NV) & 1);
+              if (ok) issue_pv(it, kt > sg.t0);
+            }
+            if (*abort_flag) ok = false;
+          }
+        }
+      } else {
+        int it = 0, qn = 0, seg = 0;  // the next P·V, the next S
+        for (; ok && more; more = sched.next(a, sg), ++seg) {
+          ok = bar_wait(q_full, seg & 1);
+          const int end = it + sg.t1 - sg.t0, begin = it;
+          // S runs up to kSBufs tiles ahead of P·V; its buffer is free once the P·V of kSBufs tiles before has read P there.
+          for (int polls = 0; ok && it < end;) {
+            const bool s_ahead = qn < end && qn < it + kSBufs &&
+                                 (qn < kSBufs || bar_test(o_done(qn % kSBufs), (qn / kSBufs - 1) & 1));
+            if (s_ahead && (qn <= it + 1 || !bar_test(p_full(it % kSBufs), (it / kSBufs) & 1)) &&
+                bar_test(k_full(qn % NS), (qn / NS) & 1)) {
+              issue_qk(qn++);
+              polls = 0;
+            } else if (qn > it && bar_test(p_full(it % kSBufs), (it / kSBufs) & 1) && bar_test(v_full(it % NV), (it / NV) & 1)) {
+              issue_pv(it, it > begin);
+              ++it;
+              polls = 0;
+            } else if (++polls > kTestPolls || *abort_flag) {
+              ok = false;
+            }
           }
         }
       }
