@@ -22,6 +22,7 @@ form a captured CUDA graph needs.
 
 from __future__ import annotations
 
+import operator
 import struct
 
 import torch
@@ -64,13 +65,20 @@ def _filled(slots) -> list:
 
 class KVSlots:
     """C-ABI views of the caches of one model (its layers), for calls that serve them all at once. Holds
-    the buffers it was built over; build it again after a cache has grown or taken a new state."""
+    the buffers it was built over; build it again after a cache has grown or taken a new state (calls with
+    views of replaced buffers are refused)."""
 
     def __init__(self, caches):
         caches = list(caches)
         if not caches:
             raise ValueError("kv_slots: no caches")
         self.buffers = [c._buffers() for c in caches]
+        if len({t.data_ptr() for bufs in self.buffers for t in bufs}) != sum(map(len, self.buffers)):
+            raise ValueError("kv_slots: a buffer is there twice: every cache once, with buffers of its own")
+        if len({c._FIRST_SLOT for c in caches}) != 1:
+            raise ValueError("kv_slots: caches of four slots beside stock ones")
+        self.caches, self._slot = caches, operator.attrgetter(caches[0]._FIRST_SLOT)
+        self._slots = [self._slot(c) for c in caches]
         first = self.buffers[0][-1]  # a row or scale buffer: its type and device are the cache's
         self.device, dtype = first.device, first.dtype
         for bufs in self.buffers:
@@ -86,6 +94,12 @@ class KVSlots:
 
     def __len__(self) -> int:
         return len(self.structs)
+
+    def check_current(self) -> None:
+        """Raises if a cache no longer has the buffers that it was viewed with."""
+        if not all(map(operator.is_, map(self._slot, self.caches), self._slots)):
+            raise ValueError("a cache has other buffers than its view (it grew, or took a new state): "
+                             "call kv_slots again")
 
 
 def kv_slots(caches) -> KVSlots:
@@ -103,6 +117,7 @@ def keep_rows(slots: KVSlots, path: torch.Tensor, accepted: torch.Tensor, base) 
     tensor of one base or one per sequence. One launch (per 64 caches), nothing is read back; afterwards the
     live rows are base + 1 + accepted[b]: with the count on the host, ``trim(T − 1 − accepted)``.
     """
+    slots.check_current()
     dev, B = slots.device, slots.batch
     for t, name in ((path, "path"), (accepted, "accepted")):
         if t.dtype != torch.int32:
@@ -130,6 +145,7 @@ def keep_rows(slots: KVSlots, path: torch.Tensor, accepted: torch.Tensor, base) 
 class MotifGroupedKVCacheBase:
     """Offset bookkeeping and storage growth shared by both 4-slot caches (``cache.py:178-300``)."""
 
+    _FIRST_SLOT = "k1"
     step = 256
 
     def update_and_fetch(self, keys, values):
@@ -492,6 +508,7 @@ class KVCache:
     every read stays below ``offset``.
     """
 
+    _FIRST_SLOT = "keys"
     step = 256
 
     def __init__(self, max_size: int | None = None):

@@ -576,6 +576,24 @@ def test_keep_rows(cuda, kind, dtype, B, H, D, n, T):
         assert all(torch.equal(x, y) for x, y in zip(bytes_of(one), bytes_of(caches[0])))
 
 
+@pytest.mark.parametrize("kind", ["rows", (4, 64), "stock"])
+def test_keep_rows_refuses_views_of_replaced_buffers(cuda, kind):
+    """A cache that grew has other buffers than its view: the call is refused and moves nothing."""
+    from mlx_motif.cache import keep_rows, kv_slots
+
+    caches = [filled(kind, 1, 2, 256, 64, "fp16", s) for s in range(3)]  # full: the next row makes it grow
+    slots = kv_slots(caches)
+    path, accepted = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([[0, 2, -1]], [1]))
+    keep_rows(slots, path, accepted, 253)
+    new = torch.zeros(1, 4 if kind == "stock" else 2, 1, 64, dtype=torch.float16, device="cuda")
+    caches[1].update_and_fetch(new, new) if kind == "stock" else caches[1].update_and_fetch_4(new, new, new, new)
+    before = [bytes_of(c) for c in caches]
+    with pytest.raises(ValueError, match="kv_slots again"):
+        keep_rows(slots, path, accepted, 253)
+    for c, was in zip(caches, before):
+        assert all(torch.equal(x, y) for x, y in zip(bytes_of(c), was))
+
+
 def test_keep_rows_many_layers_device_bases_and_stray_paths(cuda):
     """More caches than one launch takes; one base per sequence, on the device, bases outside the cache; path
     entries that are no place of the tree; counts outside it."""

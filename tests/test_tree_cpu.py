@@ -198,6 +198,21 @@ def test_keep_rows_refusals():
     with pytest.raises(ValueError, match="empty"):
         kv_slots([MotifGroupedQuantizedKVCache()])
 
+    def on_host(cls, names):
+        c = cls()
+        for name in names:
+            setattr(c, name, torch.zeros(1, 2, 256, 64, dtype=torch.float16))
+        return c
+
+    four, stock = on_host(MotifGroupedKVCache, ("k1", "k2", "v1", "v2")), on_host(KVCache, ("keys", "values"))
+    with pytest.raises(ValueError, match="twice"):  # its rows would be moved twice
+        kv_slots([four, on_host(MotifGroupedKVCache, ("k1", "k2", "v1", "v2")), four])
+    four.v2 = four.k2
+    with pytest.raises(ValueError, match="twice"):
+        kv_slots([four])
+    with pytest.raises(ValueError, match="stock"):
+        kv_slots([on_host(MotifGroupedKVCache, ("k1", "k2", "v1", "v2")), stock])
+
     structs = (N.motif_kv4_slots * 2)()
     for s in structs:
         for i in range(4):
