@@ -6,6 +6,8 @@
 // read before it is written, and a later group reads rows ≥ its own j, which no earlier one has written.
 //
 // One launch serves up to kLayers caches: their pointers travel in the kernel's parameters.
+// Bound by the launch: 3 rows of 48 fp16 layers (8 heads, D 128; 2.4 MB read and written) take 3.2 us, 8 rows of 48 q4
+// layers 5.4 us (three buffers a slot, one after the other in dependent reads of path); the bytes alone would be 0.4.
 #include "common.cuh"
 
 namespace motif {
