@@ -6,8 +6,9 @@
 // read before it is written, and a later group reads rows ≥ its own j, which no earlier one has written.
 //
 // One launch serves up to kLayers caches: their pointers travel in the kernel's parameters.
-// Bound by the launch: 3 rows of 48 fp16 layers (8 heads, D 128; 2.4 MB read and written) take 3.2 us, 8 rows of 48 q4
-// layers 5.4 us (three buffers a slot, one after the other in dependent reads of path); the bytes alone would be 0.4.
+// Bound by the launch: 3 rows of 48 fp16 layers (8 heads, D 128; 2.4 MB read and written) take 2.8 us, 8 rows of 48 q4
+// layers 4.1 us; the bytes alone would be 0.4. A CTA moves one buffer of a slot's head (codes, scales and biases one
+// after the other: 5.2 us); packed rows are short, and CTAs of 64 threads all run at once there (of 128: 5.1 us).
 #include "common.cuh"
 
 namespace motif {
@@ -38,7 +39,7 @@ template <typename U>
 __device__ __forceinline__ void move_rows(U* rows, int per_row, const int32_t* path, int n, int64_t cap_left, int T) {
   const int tid = threadIdx.x;
   // units of rows 1..n in order, one per thread and group
-  for (int i0 = 0; i0 < n * per_row; i0 += kKeepThreads) {
+  for (int i0 = 0; i0 < n * per_row; i0 += blockDim.x) {
     const int i = i0 + tid;
     const int j = 1 + i / per_row, c = i % per_row;
     U v{};
@@ -62,16 +63,15 @@ __global__ void __launch_bounds__(kKeepThreads) keep_rows_kernel(const __grid_co
   if (n <= 0 || base < 0 || base >= a.limit) return;
   const int64_t left = a.limit - base;  // rows of the tree that the cache holds
   const int32_t* path = a.path + b * a.path_b;
-  for (int k = 0; k < a.parts; ++k) {
-    char* p = static_cast<char*>(a.ptr[layer][slot][k]) + ((int64_t)head * a.cap + base) * a.row_bytes[k];
-    const int per = a.row_bytes[k] / a.unit[k];
-    const int m = (int)min((int64_t)n, left - 1);
-    switch (a.unit[k]) {
-      case 16: move_rows(reinterpret_cast<uint4*>(p), per, path, m, left, a.T); break;
-      case 8: move_rows(reinterpret_cast<uint2*>(p), per, path, m, left, a.T); break;
-      case 4: move_rows(reinterpret_cast<uint32_t*>(p), per, path, m, left, a.T); break;
-      default: move_rows(reinterpret_cast<uint16_t*>(p), per, path, m, left, a.T); break;
-    }
+  const int k = blockIdx.z;
+  char* p = static_cast<char*>(a.ptr[layer][slot][k]) + ((int64_t)head * a.cap + base) * a.row_bytes[k];
+  const int per = a.row_bytes[k] / a.unit[k];
+  const int m = (int)min((int64_t)n, left - 1);
+  switch (a.unit[k]) {
+    case 16: move_rows(reinterpret_cast<uint4*>(p), per, path, m, left, a.T); break;
+    case 8: move_rows(reinterpret_cast<uint2*>(p), per, path, m, left, a.T); break;
+    case 4: move_rows(reinterpret_cast<uint32_t*>(p), per, path, m, left, a.T); break;
+    default: move_rows(reinterpret_cast<uint16_t*>(p), per, path, m, left, a.T); break;
   }
 }
 
@@ -148,7 +148,7 @@ int motif_kv4_keep_rows(int dtype, const motif_kv4_slots* caches, int64_t n_cach
       a.unit[k] = bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : 2;
       MOTIF_REQUIRE(bits % 2 == 0, MOTIF_ERR_BAD_CONTRACT, "keep_rows: misaligned cache");
     }
-    keep_rows_kernel<<<dim3((unsigned)(4 * n), (unsigned)a.heads), kKeepThreads, 0, as_stream(stream)>>>(a);
+    keep_rows_kernel<<<dim3((unsigned)(4 * n), (unsigned)a.heads, (unsigned)a.parts), a.parts == 1 ? kKeepThreads : kKeepThreads / 2, 0, as_stream(stream)>>>(a);
     const int rc = check_launch("keep_rows");
     if (rc) return rc;
   }
