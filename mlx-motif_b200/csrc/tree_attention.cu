@@ -422,7 +422,7 @@ struct TcMap {  // shared memory, bytes from a 1024-byte boundary
   static constexpr int kV = kK + TcCfg<BITS>::kStages * kKBytes;
   static constexpr int kVBytes = 2 * kKBytes;
   static constexpr int kBar = kV + TcCfg<BITS>::kVStages * kVBytes;
-  static constexpr int kNumBars = 1 + 2 * TcCfg<BITS>::kStages + 2 * TcCfg<BITS>::kVStages + 3 * kSBufs + 1 + 2 * kRawMax + 12;
+  static constexpr int kNumBars = 1 + 2 * TcCfg<BITS>::kStages + 2 * TcCfg<BITS>::kVStages + 3 * kSBufs + 1 + 2 * kRawMax + 13;
   static constexpr int kState = kBar + kNumBars * 8 + 16;  // [128] reference maxima, [2][128] sums of the groups
   static constexpr int kJoin = kState + 3 * kTR * 4;       // [128] (maximum, sum) of this CTA's part, its rows' weights
   static constexpr int kBad = kJoin + kTR * 8 + (kTR + 2 * kMaxCluster) * 4;        // drafted rows cleared: [2 segments][8 warps] Cleared
@@ -671,6 +671,7 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
   auto raw_empty = [&](int s) { return bar + 8u * (kB3 + kRawMax + s); };
   auto m_next = [&](int g, int q) { return bar + 8u * (kB4 + 4 * g + q); };  // maxima handed on by group g
   auto l_both = [&](int q) { return bar + 8u * (kB4 + 8 + q); };
+  const uint32_t o_read = bar + 8u * (kB4 + 12);  // every softmax warp has read its part of a segment's O and sums
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Map::kBar + Map::kNumBars * 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -704,19 +705,19 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
     }
   };
   if (softmax && more) fetch_q(sg);
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < Map::kNumBars; ++i) {
-      int count = 1;
-      if (i == 0) count = 8;                                                                  // q_full
-      if ((i >= 1 && i < 1 + NS) || (i >= kB0 && i < kB0 + NV)) count = Cfg::kFill;           // k_full, v_full
-      if (i >= kB2 && i < kB2 + kSBufs) count = 4;                                            // p_full
-      if (i >= kB3 + kRawMax && i < kB4) count = Cfg::kFill;                                  // raw_empty
-      if (i >= kB4 + 8) count = 2;                                                            // l_both
-      if (i == kB2 + 2 * kSBufs) count = BITS == 16 ? 2 : 1;                                  // drain
-      tc::mbar_init(bar + 8u * i, count);
-    }
-    *abort_flag = 0;
-    for (int i = 0; i < 16; ++i) reinterpret_cast<Cleared*>(smem + Map::kBad)[i].seg = -1;
+  if (threadIdx.x < Map::kNumBars) {  // a barrier a thread: one thread's loop over all takes 1 us
+    const int i = threadIdx.x;
+    int count = 1;
+    if (i == 0) count = 8;                                                                  // q_full
+    if ((i >= 1 && i < 1 + NS) || (i >= kB0 && i < kB0 + NV)) count = Cfg::kFill;           // k_full, v_full
+    if (i >= kB2 && i < kB2 + kSBufs) count = 4;                                            // p_full
+    if (i >= kB3 + kRawMax && i < kB4) count = Cfg::kFill;                                  // raw_empty
+    if (i >= kB4 + 8 && i < kB4 + 12) count = 2;                                            // l_both
+    if (i == kB4 + 12) count = 8;                                                           // o_read
+    if (i == kB2 + 2 * kSBufs) count = BITS == 16 ? 2 : 1;                                  // drain
+    tc::mbar_init(bar + 8u * i, count);
+    if (i < 16) reinterpret_cast<Cleared*>(smem + Map::kBad)[i].seg = -1;
+    if (i == 0) *abort_flag = 0;
     tc::mbar_fence_init();
   }
   float2* join_ml = reinterpret_cast<float2*>(smem + Map::kJoin);
@@ -821,7 +822,8 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
         // as much again between them: 1.15 us a tile from one thread).
         int it = 0, seg = 0;
         for (; ok && more; more = sched.next(a, sg), ++seg) {
-          if (warp == 1) ok = bar_wait(q_full, seg & 1);
+          // A segment's first P·V overwrites O, which both groups read after they met in l_both.
+          if (warp == 1 || seg) ok = bar_wait(warp == 1 ? q_full : o_read, (warp == 1 ? seg : seg + 1) & 1);
           for (int kt = sg.t0; ok && kt < sg.t1; ++kt, ++it) {
             if (warp == 1) {  // S: its buffer is free once the P·V of kSBufs tiles before has read P there
               ok = (it < kSBufs || bar_wait(o_done(it % kSBufs), (it / kSBufs - 1) & 1)) && bar_wait(k_full(it % NS), (it / NS) & 1);
@@ -846,7 +848,8 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
                 bar_test(k_full(qn % NS), (qn / NS) & 1)) {
               issue_qk(qn++);
               polls = 0;
-            } else if (qn > it && bar_test(p_full(it % kSBufs), (it / kSBufs) & 1) && bar_test(v_full(it % NV), (it / NV) & 1)) {
+            } else if (qn > it && (it > begin || bar_test(o_read, (seg + 1) & 1)) &&  // O as above; before the first phase the parity of a finished one
+                       bar_test(p_full(it % kSBufs), (it / kSBufs) & 1) && bar_test(v_full(it % NV), (it / NV) & 1)) {
               issue_pv(it, it > begin);
               ++it;
               polls = 0;
@@ -1098,6 +1101,11 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
           add_cleared<T, D, BITS>(a, sg.b, sg.g, bad, seg, pr, t, ctx, m_ref, inv, grp,
                                   sg.slot < 0 ? static_cast<T*>(a.y) + row * 2 * D : nullptr, sg.slot, r, smem + Map::kK);
       }
+      // This warp's last read of the segment's O (and of l_row: the next sums are written after the next segment's
+      // P·V) is over. Every softmax warp arrives, with a row or without.
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(o_read);
       if (!alive) *abort_flag = 1;
       sg = nx;
       ++seg;
