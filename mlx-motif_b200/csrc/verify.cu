@@ -245,6 +245,9 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyArgs a)
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int b = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool greedy = a.inv_t == 0.0;
+  // Another CTA's shared memory may be written once that CTA has started: everyone arrives here and waits below,
+  // behind the row laws.
+  if (C > 1) asm volatile("barrier.cluster.arrive.relaxed;\n" ::: "memory");
   unsigned long long* top = reinterpret_cast<unsigned long long*>(dyn);  // τ = 0: a row's largest entry; in place of …
   float* pm = reinterpret_cast<float*>(dyn);                             // … the row's target law: maximum, 1 / Σ
   float* pz = pm + a.T;
@@ -435,6 +438,7 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyArgs a)
     exact = true;
   };
 
+  if (C > 1) asm volatile("barrier.cluster.wait;\n" ::: "memory");  // every CTA of the cluster has started
   int cur = 0, kept = 1;
   if (rank == 0 && tid == 0) path[0] = 0;
   for (int i = first[0]; i >= 0;) {
