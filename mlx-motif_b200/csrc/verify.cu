@@ -36,6 +36,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "sweep.cuh"
 
 namespace motif {
 namespace {
@@ -69,26 +70,6 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// exp((l − m)·inv_t) for the sweeps over a row, by a table of 2^(j/256) (Tang, "Table-driven implementation of the
-// exponential function in IEEE floating-point arithmetic", ACM TOMS 15, 1989): y = (l − m)·inv_t·log2 e =
-// n/256 + f, |f| ≤ 2^-9, 2^f by its series to f⁴ (the next term is 4·10^-17); nine 64-bit operations, within 2^-50
-// of exp for |y| ≤ 60 (y's own rounding). Below 2^-1022: 0. k = inv_t·log2 e, mk = m·k of a finite m.
-constexpr int kTable = 256;
-__device__ __forceinline__ double sweep_weight(float l, double k, double mk, const double* table) {
-  const double y = fma((double)l, k, -mk);
-  constexpr double kMagic = 6755399441055744.0 / kTable;  // 1.5·2^52 / 256: the sum rounds y to 1/256
-  const double t = y + kMagic;
-  const int n = __double2loint(t);
-  const double f = y - (t - kMagic);
-  double q = fma(f, 0.0096181291076284772, 0.055504108664821580);  // (ln 2)^i / i!
-  q = fma(f, q, 0.24022650695910071);
-  q = fma(f, q, 0.69314718055994531);
-  const double s = table[n & (kTable - 1)];
-  const double e = fma(s * f, q, s);
-  const int hi = __double2hiint(e) + ((n >> 8) << 20);
-  return y >= -1022.0 ? __hiloint2double(hi, __double2loint(e)) : 0.0;
-}
-
 // Order-preserving key of (value, index): the larger value, then the smaller index.
 __device__ __forceinline__ unsigned long long top_key(float v, int i) {
   uint32_t b = __float_as_uint(v + 0.f);  // −0 ties with 0
@@ -239,7 +220,7 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyArgs a)
   namespace cg = cooperative_groups;
   extern __shared__ __align__(16) uint8_t dyn[];
   __shared__ double ws[kWalkWarps], sums[2][kMaxCluster][2];
-  __shared__ double scan[kWalkWarps], table[kTable];
+  __shared__ double scan[kWalkWarps], table[kSweepTable];
   __shared__ int found;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -274,7 +255,7 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyArgs a)
     px[i] = pa >= 0 ? logit(P + pa * a.pr, x) : 0.f;
     qx[i] = pa >= 0 ? logit(Q + pa * a.qr, x) : 0.f;
   }
-  if (!greedy && tid < kTable) table[tid] = exp2(tid / (double)kTable);
+  if (!greedy && tid < kSweepTable) table[tid] = exp2(tid / (double)kSweepTable);
   __syncthreads();
   // links: a warp finds a row's children, 32 rows a ballot, from the last to the first
 #pragma unroll 1
@@ -376,7 +357,7 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyArgs a)
   int phase = 0;
   // exp((l − m)/τ); an infinite maximum's entries share the law, a row of -inf has none
   auto entry = [&](float l, float m) {
-    const double e = sweep_weight(l, k, (double)m * k, table);
+    const double e = sweep_weight(l, (double)m, k, table);
     return fabsf(m) < INFINITY ? e : m > 0.f && l == m ? 1.0 : 0.0;
   };
   // Sums of two values over the cluster, the same on every CTA; my warps' sums of the first stay in ws.

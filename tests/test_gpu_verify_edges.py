@@ -24,3 +24,35 @@ def test_walks_in_a_row(cuda, V, T):
     got = [speculative_verify(*dev, 0.8) for _ in range(100)]
     for r in got:
         same(r, want)
+
+
+LOWEST = {"fp32": torch.finfo(torch.float32).min, "bf16": float(torch.finfo(torch.bfloat16).min), "fp16": -65504.0}
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("temp", [1e-6, 0.3, 0.5, 0.7, 1.0, 1.3, 50.0, 1e6])
+@pytest.mark.parametrize("V", [300, 40000])
+def test_rows_of_very_large_logits(cuda, dtype, temp, V):
+    """A row of the type's lowest value throughout is the uniform law; maxima of ±1e20 (16-bit types: near their
+    ends) are one token's or share the law; the residual of such rows."""
+    from mlx_motif.kernels import speculative_verify_reference
+
+    B, T = 6, 3
+    tok, par, p, q, u = drafts(V, B, T, V, dtype, tree=False)
+    low, big = LOWEST[dtype], {"fp32": 1e20, "bf16": 1e20, "fp16": 60000.0}[dtype]
+    p[0, 0] = low
+    q[1] = low
+    p[2], q[2] = low, low
+    p[3, 0, 7], p[3, 1, [11, 250]] = big, big
+    q[3, 0, 7] = big
+    p[4] -= big
+    q[4] -= big
+    p[5], q[5] = p[5] + big, q[5] + big
+    p[5, 0, ::3] = low
+    want = speculative_verify_reference(tok, par, p, q, u, temp)
+    same(verify(tok, par, p, q, u, temp), want)
+    alone = [t[:1, :1].contiguous() for t in (tok, par, p, q, u)]  # the draw alone
+    for x in (0.0, 0.25, 0.5, 0.999):
+        alone[4].fill_(x)
+        r = verify(*alone, temp)
+        assert r.next_token.item() == int(x * V), (x, r.next_token.item())
