@@ -594,7 +594,8 @@ MOTIF_API int motif_speculative_accept(const void* p_logits, const void* q_logit
  * uniforms[b, i]: accepted with probability min(1, w(x) / q(x)), w = p and
  * after each rejection max(0, w - q) renormalised; an accepted child becomes
  * the current row. next_token is drawn from the last w by inverting its
- * running sum at uniforms[b, 0]: the tokens follow the target's law. Temperature
+ * running sum at uniforms[b, 0]: the tokens follow the target's law (uniforms in
+ * [0, 1); from 1 on it is the last token with weight). Temperature
  * is 0 or in [1e-6, 1e6]. At 0: a child is accepted if it is the target's argmax, next_token = the argmax
  * (first index on ties); q_logits and uniforms may be NULL. A token outside
  * [0, vocab) is never accepted (padding); NaN logits count as -inf; a target

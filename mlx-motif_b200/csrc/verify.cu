@@ -468,26 +468,30 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyArgs a)
     total(s, 0.0, W, unused);
   }
   auto w = [&](int e) { return plain ? at_p(p, e) : fmax(0.0, at_p(p, e) * izp - coef * (at_q(q, e) * izq)); };
-  // the CTA, then the warp's range that holds the border; the last one with any weight if rounding leaves none beyond it
-  const double target = (double)u[0] * W;
-  double before = 0.0;
+  // the CTA, then the warp's range that holds the border; the last one with any weight if none goes beyond it (u_0 ≥ 1,
+  // or rounding). `before`: the weights in front of it
+  const double target = u[0] < 1.f ? (double)u[0] * W : INFINITY;
+  double before = 0.0, upto = 0.0;
   int cta = -1, sub = -1;
   for (int c = 0; c < C; ++c) {
     const double x = sums[phase ^ 1][c][0];
     if (!(x > 0.0)) continue;
     cta = c;
-    if (before + x > target) break;
-    before += x;
+    before = upto;
+    upto += x;
+    if (upto > target) break;
   }
   if (cta < 0) {  // a row without a finite logit
     if (rank == 0 && tid == 0) a.next[b] = 0;
   } else if (cta == rank) {
+    upto = before;
     for (int k = 0; k < kWalkWarps; ++k) {
       const double x = ws[k];
       if (!(x > 0.0)) continue;
       sub = k;
-      if (before + x > target) break;
-      before += x;
+      before = upto;
+      upto += x;
+      if (upto > target) break;
     }
     const int e0 = range(sub), e1 = range(sub + 1), per = (e1 - e0 + kWalkThreads - 1) / kWalkThreads;
     const int mine0 = min(e0 + tid * per, e1), mine1 = min(mine0 + per, e1);
@@ -522,7 +526,7 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyArgs a)
     __syncthreads();
     const bool none = found == 0x7fffffff;
     __syncthreads();
-    if (none) {  // u_0 at or beyond the end
+    if (none) {  // nothing beyond the target: the last entry with weight
       if (tid == 0) found = -1;
       __syncthreads();
       if (last >= 0) atomicMax(&found, last);

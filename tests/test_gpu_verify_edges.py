@@ -56,3 +56,28 @@ def test_rows_of_very_large_logits(cuda, dtype, temp, V):
         alone[4].fill_(x)
         r = verify(*alone, temp)
         assert r.next_token.item() == int(x * V), (x, r.next_token.item())
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16"])
+@pytest.mark.parametrize("V", [5, 300, 4097, 70000])  # within a warp's range, one CTA, several
+def test_draws_at_the_ends(cuda, dtype, V):
+    """u_0 of 1, or beyond, draws the last token with weight, 0 the first one; with the law's ends masked, after
+    rejections too."""
+    from mlx_motif.kernels import speculative_verify_reference
+
+    B, T = 4, 3
+    tok, _, p, q, u = drafts(V, B, T, V, dtype, tree=False, apart=2.0)
+    par = torch.tensor([-1, 0, 0], dtype=torch.int32)
+    q = q[:, :1].contiguous()
+    g = torch.Generator().manual_seed(V)
+    tok[:, 1:] = torch.multinomial(torch.softmax(q[:, 0].double(), -1), 2, replacement=True, generator=g).int()
+    p[1, :, -(V // 3) - 1 :] = -float("inf")
+    p[2, :, : V // 2] = -float("inf")
+    for u0 in (1.0, 1.5, 1.0 - 2.0**-24, 0.0):
+        for rest in (0.0, 0.5, 1.0):
+            u.fill_(rest)
+            u[:, 0] = u0
+            want = speculative_verify_reference(tok, par, p, q, u, 0.9)
+            same(verify(tok, par, p, q, u, 0.9), want)
+            if u0 >= 1.0 and want.accepted[1]:
+                assert want.next_token[1] == V - V // 3 - 2
