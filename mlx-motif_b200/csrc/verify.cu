@@ -44,9 +44,14 @@ namespace {
 constexpr int kChunk = 8192, kStatThreads = 256;
 constexpr int kWalkThreads = 512, kWalkWarps = kWalkThreads / 32;
 constexpr int kMaxRows = 1024, kMaxCluster = 16;
-// The 32-bit row sums are within 2^-17 (exponent's rounding at |x| ≤ 60: 2^-18; 64 additions: 2^-18). A test closer
-// to its border than this is repeated with sums in 64 bits, both rows added in the same order.
-constexpr float kMargin = 1.f / 32768;
+// A test in 32 bits that is closer to its border u·q = p than (kMargin + chunks·kMarginChunk)·(p + q) + kMarginTiny is
+// repeated with sums in 64 bits, both rows added in the same order. In steps of 2^-24 relative, an exponential 2^x has 5
+// roundings of its exponent (l − m, 1/τ, log2 e, their product, the product with l − m), ln 2·|x| each: 409 for
+// |x| ≤ 118, and 4 of its own. The row's sum: its exponentials weigh themselves, so that |x| counts by its mean, at most
+// log2 of the vocabulary, 30 (104); 23 additions within a chunk; chunks/8 additions and chunks/32 + 4 changes of the
+// maximum, 4 each, over the chunks. With the quotient and products less than 600 + chunks/4. Below 2^-118 a
+// probability may be anything down to 0 (2^-126 and less is flushed): there kMarginTiny decides.
+constexpr float kMargin = 1.f / (1 << 14), kMarginChunk = 1.f / (1 << 26), kMarginTiny = 0x1p-100f;
 
 struct VerifyArgs {
   const void *p, *q;
@@ -354,6 +359,7 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyArgs a)
   float mp = pm[0], mq = 0.f;
   double izp = 1.0, izq = 1.0, coef = 0.0, S = 1.0;
   bool exact = false;
+  const float margin = kMargin + a.chunks * kMarginChunk;
   int phase = 0;
   // exp((l − m)/τ); an infinite maximum's entries share the law, a row of -inf has none
   auto entry = [&](float l, float m) {
@@ -431,7 +437,7 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(VerifyArgs a)
       auto prob = [&](float l, float m, float iz) { return l == m ? iz : ex2((l - m) * kf) * iz; };
       const float pe = prob(px[i], mp, pz[cur]), qe = prob(qx[i], mq, qz[cur]), ue = u[i] * qe;
       ok = ue < pe;
-      sure = fabsf(ue - pe) > kMargin * (pe + qe);
+      sure = fabsf(ue - pe) > margin * (pe + qe) + kMarginTiny;
     }
     if (!sure) {
       if (!exact) make_exact(p, q);

@@ -81,3 +81,27 @@ def test_draws_at_the_ends(cuda, dtype, V):
             same(verify(tok, par, p, q, u, 0.9), want)
             if u0 >= 1.0 and want.accepted[1]:
                 assert want.next_token[1] == V - V // 3 - 2
+
+
+@pytest.mark.parametrize("temp", [0.7, 1.0])
+@pytest.mark.parametrize("V", [50, 40000])
+def test_drafts_of_tiny_probability(cuda, temp, V):
+    """Drafted tokens whose probabilities leave the 32-bit range (2^-126) in one row or both: accepted or not by
+    their quotient."""
+    from mlx_motif.kernels import speculative_verify_reference
+
+    B, T = 24, 2
+    g = torch.Generator().manual_seed(V)
+    p, q = torch.randn((B, T, V), generator=g), torch.randn((B, 1, V), generator=g)
+    p[:, :, 0], q[:, :, 0] = 20.0, 20.0
+    tok = torch.full((B, T), 7, dtype=torch.int32)
+    par = torch.tensor([-1, 0], dtype=torch.int32)
+    ln2 = 0.6931471805599453
+    u = torch.empty((B, T)).fill_(0.3)
+    for b in range(B):
+        at = -120.0 - b % 12  # log2 of the draft's probability, about; the target's is 0.8 or 3 below it
+        q[b, 0, 7] = 20.0 + at * ln2 * temp
+        p[b, 0, 7] = 20.0 + (at - (0.8 if b < 12 else 3.0)) * ln2 * temp
+    want = speculative_verify_reference(tok, par, p, q, u, temp)
+    assert want.accepted.tolist() == [1] * 12 + [0] * 12
+    same(verify(tok, par, p, q, u, temp), want)
