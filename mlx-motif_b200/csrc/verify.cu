@@ -551,6 +551,31 @@ constexpr size_t kRoom = 224 * 1024;  // dynamic shared memory beside the walk's
 
 int chunks_of(int64_t V) { return (int)ceil_div(V, kChunk); }
 
+// Clusters of 16 CTAs need a part of the GPU with 16 free SMs where a CTA takes the most shared memory that a call asks
+// for (smaller calls share SMs): asked for that size, once per device. The kernel's attributes are set.
+template <typename T>
+bool clusters_of_16() {
+  static std::atomic<int> known[64]{};  // 0: not asked, 1: they fit, 2: they do not
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  if (dev < 64 && known[dev] != 0) return known[dev] == 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(16);
+  cfg.blockDim = dim3(kWalkThreads);
+  cfg.dynamicSmemBytes = kRoom;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = 16;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  int n = 0;
+  const bool fit = cudaOccupancyMaxActiveClusters(&n, verify_walk_kernel<T, true>, &cfg) == cudaSuccess && n > 0;
+  (void)cudaGetLastError();
+  if (dev < 64) known[dev] = fit ? 1 : 2;
+  return fit;
+}
+
 template <typename T>
 int launch_verify(const VerifyArgs& a, int64_t batch, cudaStream_t st) {
   const bool greedy = a.inv_t == 0.0;
@@ -589,21 +614,13 @@ int launch_verify(const VerifyArgs& a, int64_t batch, cudaStream_t st) {
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  if (C > 8) {  // clusters of 16 need a part of the GPU with 16 SMs: asked once
-    static std::atomic<int> fits{-1};
-    if (fits < 0) {
-      int n = 0;
-      fits = cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess && n > 0;
-      (void)cudaGetLastError();
-    }
-    if (!fits) {
-      C = 8;
-      cfg.gridDim = dim3((unsigned)(batch * C));
-      at[1].val.clusterDim.x = 8;
-      cache = bytes(C) <= kRoom;
-      kern = cache ? verify_walk_kernel<T, true> : verify_walk_kernel<T, false>;
-      cfg.dynamicSmemBytes = cache ? bytes(C) : rows;
-    }
+  if (C > 8 && !clusters_of_16<T>()) {
+    C = 8;
+    cfg.gridDim = dim3((unsigned)(batch * C));
+    at[1].val.clusterDim.x = 8;
+    cache = bytes(C) <= kRoom;
+    kern = cache ? verify_walk_kernel<T, true> : verify_walk_kernel<T, false>;
+    cfg.dynamicSmemBytes = cache ? bytes(C) : rows;
   }
   e = cudaLaunchKernelEx(&cfg, kern, a);
   if (e != cudaSuccess) return fail(MOTIF_ERR_CUDA, "speculative_verify: %s", cudaGetErrorString(e));

@@ -4,6 +4,11 @@ whole numbers, which have to be equal. The drafts are ``test_gpu_tree.py``'s.
 
 from __future__ import annotations
 
+import os
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 from test_gpu_tree import drafts, same, verify
@@ -105,3 +110,19 @@ def test_drafts_of_tiny_probability(cuda, temp, V):
     want = speculative_verify_reference(tok, par, p, q, u, temp)
     assert want.accepted.tolist() == [1] * 12 + [0] * 12
     same(verify(tok, par, p, q, u, temp), want)
+
+
+def test_a_small_call_says_nothing_about_a_large_one(cuda):
+    """In a fresh process: a vocabulary whose clusters share SMs, then one whose CTAs take an SM's shared memory."""
+    code = """
+import torch
+from test_gpu_tree import drafts, same, verify
+from mlx_motif.kernels import speculative_verify_reference
+for V in (32768, 219520, 32768):
+    for dtype in ("fp16", "fp32"):
+        args = drafts(V, 1, 4, V, dtype, tree=False)
+        same(verify(*args, 0.7), speculative_verify_reference(*args, 0.7))
+"""
+    here = Path(__file__).resolve().parent
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join([str(here), str(here.parent / "mlx-motif_b200"), str(here.parent)]))
+    subprocess.run([sys.executable, "-c", code], check=True, env=env, timeout=300)
