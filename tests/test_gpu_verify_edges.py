@@ -126,3 +126,21 @@ for V in (32768, 219520, 32768):
     here = Path(__file__).resolve().parent
     env = dict(os.environ, PYTHONPATH=os.pathsep.join([str(here), str(here.parent / "mlx-motif_b200"), str(here.parent)]))
     subprocess.run([sys.executable, "-c", code], check=True, env=env, timeout=300)
+
+
+@pytest.mark.parametrize("B,T,V,tree,dtype", [
+    (9, 3, 219520, False, "fp16"),  # nine sequences: clusters of 8, more than shared memory holds
+    (1, 4, 256000, False, "bf16"),  # one CTA's sixteenth of the vocabulary does not fit
+    (1, 300, 219520, True, "fp16"),  # the rows' records leave no room
+    (2, 5, 500001, True, "fp32"),
+])
+@pytest.mark.parametrize("temp", [0.7, 1.0])
+def test_walks_without_kept_exponentials(cuda, B, T, V, tree, dtype, temp):
+    """Vocabularies whose exponentials do not fit the cluster's shared memory: every sweep computes them again."""
+    from mlx_motif.kernels import speculative_verify_reference
+
+    args = drafts(B + T, B, T, V, dtype, tree, apart=1.5)
+    want = speculative_verify_reference(*args, temp)
+    same(verify(*args, temp), want)
+    hard = args[4].clone().fill_(0.999)  # rejections at every row
+    same(verify(*args[:4], hard, temp), speculative_verify_reference(*args[:4], hard, temp))
