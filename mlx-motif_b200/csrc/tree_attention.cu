@@ -1316,7 +1316,7 @@ int sm_count() {  // of the first device asked for: a machine's GPUs are alike
   return n;
 }
 
-constexpr int64_t kMaxTreeRows = 256;
+constexpr int64_t kMaxTreeRows = 256, kMaxCap = 1 << 30, kMaxBatch = 1 << 20, kMaxHeads = 1 << 16;
 
 // Shared memory of the K and V tiles, which a cluster's join takes over.
 int join_room(int bits, int64_t D) {
@@ -1467,11 +1467,13 @@ extern "C" {
 size_t motif_sdpa_dual_v_tree_workspace_bytes(int dtype, int bits, int group_size, int64_t batch, int64_t h_q,
                                               int64_t h_kv, int64_t tree_rows, int64_t kv_cap, int64_t head_dim,
                                               int64_t kv_len_bound, int one_length) {
-  if (batch < 1 || h_q < 1 || h_kv < 1 || tree_rows < 1 || kv_cap < 1 || head_dim < 1 || group_size < 1 ||
+  // a call of other sizes is refused
+  if (batch < 1 || batch >= kMaxBatch || h_q < 1 || h_q >= kMaxHeads || h_kv < 1 || h_q % h_kv != 0 || tree_rows < 1 ||
+      tree_rows > kMaxTreeRows || kv_cap < 1 || kv_cap >= kMaxCap || head_dim < 1 || head_dim > 128 || group_size < 1 ||
       head_dim < group_size)
     return 0;
-  return make_plan(dtype, bits, group_size, batch, h_kv, h_q / h_kv * tree_rows, head_dim, kv_cap, kv_len_bound,
-                   one_length != 0).bytes;
+  return make_plan(dtype, bits, group_size, batch, h_kv, h_q / h_kv * tree_rows, head_dim, kv_cap,
+                   kv_len_bound < kv_cap ? kv_len_bound : kv_cap, one_length != 0).bytes;
 }
 
 int motif_sdpa_dual_v_tree(int dtype, int bits, int group_size, const void* q, const motif_tree_kv* kv,
@@ -1483,8 +1485,8 @@ int motif_sdpa_dual_v_tree(int dtype, int bits, int group_size, const void* q, c
   MOTIF_REQUIRE(dtype == MOTIF_F16 || dtype == MOTIF_BF16 || dtype == MOTIF_F32, MOTIF_ERR_DTYPE,
                 "sdpa_dual_v_tree: unsupported dtype code %d", dtype);
   MOTIF_REQUIRE(bits == 16 || bits == 4 || bits == 8, MOTIF_ERR_DTYPE, "sdpa_dual_v_tree: bits %d (4, 8 or 16)", bits);
-  MOTIF_REQUIRE(batch > 0 && h_q > 0 && h_kv > 0 && kv_cap > 0 && kv_cap < (1ll << 30) && batch < (1 << 20) &&
-                    h_q < (1 << 16),
+  MOTIF_REQUIRE(batch > 0 && h_q > 0 && h_kv > 0 && kv_cap > 0 && kv_cap < kMaxCap && batch < kMaxBatch &&
+                    h_q < kMaxHeads,
                 MOTIF_ERR_BAD_SHAPE, "sdpa_dual_v_tree: bad shape B=%lld H_q=%lld H_kv=%lld cap=%lld", (long long)batch,
                 (long long)h_q, (long long)h_kv, (long long)kv_cap);
   MOTIF_REQUIRE(tree_rows >= 1 && tree_rows <= kMaxTreeRows, MOTIF_ERR_BAD_CONTRACT,
