@@ -73,7 +73,7 @@ constexpr int kLead = 8, kLeadTiles = 8;
 
 struct Line {
   int total, per, rem, grid, lead;
-  __device__ __forceinline__ void init(int tiles, int units, int parts) {  // tiles of all units < 2^28: checked by the host
+  __device__ __forceinline__ void init(int tiles, int units, int parts) {  // tiles + kLead·units < 2^31: checked by the host
     grid = parts;
     lead = tiles >= kLeadTiles * grid ? kLead : 0;
     total = tiles + units * lead;
@@ -1333,6 +1333,7 @@ struct Plan {
   int cuts;       // parts of every unit, or 0: the line
   bool cluster;   // joined by the cluster of a unit's CTAs, without a second launch
   int64_t tiles;  // key tiles of all units at the longest lengths
+  int64_t line;   // length of the line at most
   int64_t grid;   // CTAs: at most as many as run at once
   size_t ml_offset, bytes;
 };
@@ -1351,6 +1352,7 @@ Plan make_plan(int dtype, int bits, int gs, int64_t B, int64_t HKV, int64_t R, i
   const int64_t ctas = (p.tc ? 1 : 2) * (int64_t)sm_count();
   const int64_t nt = ceil_div(len_bound < 1 ? 1 : len_bound, p.tile_keys), units = B * HKV * p.row_tiles;
   p.tiles = nt * units;
+  p.line = p.tiles + kLead * units;
   p.grid = p.tiles < ctas ? p.tiles : ctas;
   int64_t parts = 2 * p.grid;
   if ((one_length || B == 1) && units <= ctas && B < 65536 && HKV * p.row_tiles < 65536) {
@@ -1370,7 +1372,8 @@ Plan make_plan(int dtype, int bits, int gs, int64_t B, int64_t HKV, int64_t R, i
         const double t = 0.9 * ceil_div(nt, k) + 3.5;
         if (t < best) best = t, c = k, p.cluster = true;
       }
-    if (p.cluster || c < most || most == nt || 8 * c * units >= 7 * ctas) {
+    // cut_at multiplies in 32 bits: a longer cache is a line
+    if (c * nt < (1ll << 32) && (p.cluster || c < most || most == nt || 8 * c * units >= 7 * ctas)) {
       p.cuts = (int)c;
       parts = p.cluster || c == 1 ? 0 : c * units;
     }
@@ -1555,8 +1558,8 @@ int motif_sdpa_dual_v_tree(int dtype, int bits, int group_size, const void* q, c
   a.slot_rows = p.slot_rows;
   a.cuts = p.cuts;
   a.cluster = p.cluster;
-  MOTIF_REQUIRE(p.tiles < (1ll << 28), MOTIF_ERR_BAD_SHAPE, "sdpa_dual_v_tree: %lld key tiles in one call",
-                (long long)p.tiles);
+  MOTIF_REQUIRE(p.tiles < (1ll << 28) && p.line < (1ll << 31), MOTIF_ERR_BAD_SHAPE,
+                "sdpa_dual_v_tree: %lld key tiles in one call", (long long)p.tiles);
   MOTIF_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes), MOTIF_ERR_WORKSPACE,
                 "sdpa_dual_v_tree: workspace of %zu bytes, needs %zu", workspace_bytes, p.bytes);
   MOTIF_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, MOTIF_ERR_BAD_CONTRACT,
