@@ -244,8 +244,8 @@ MOTIF_API int motif_vanilla_decode_step(const void* qkv, const float* inv_freq, 
  * workspace: motif_sdpa_dual_v_tree_workspace_bytes of the same arguments
  * (kv_len_bound: kv_len, or kv_cap with kv_len_dev; one_length: 0 with
  * kv_len_stride 1, else 1; may be 0), any contents; calls that may overlap
- * need one each. err (optional device int): set to 1 if a
- * pipeline wait timed out (the rows it concerns are then NaN). */
+ * need one each. err (optional int, device or pinned host memory): set to 1
+ * if a pipeline wait timed out (the rows it concerns are then NaN). */
 typedef struct motif_tree_kv {
   const void* data[3];
   const void* scales[3];

@@ -1182,7 +1182,7 @@ __global__ void __launch_bounds__(TcCfg<BITS>::kThreads, 1) tree_tc_kernel(const
     tc::tmem_dealloc(tmem, kCols);
   }
   if (a.cluster) join_cluster<T, D>(a, smem + Map::kK, join_ml, reinterpret_cast<float*>(join_ml + kTR));
-  if (threadIdx.x == 0 && *abort_flag && a.err) atomicExch(a.err, 1);
+  if (threadIdx.x == 0 && *abort_flag && a.err) *reinterpret_cast<volatile int*>(a.err) = 1;  // may be host memory
 }
 
 // ---- join of the cut units' partials -----------------------------------------------------------------

@@ -8,6 +8,7 @@ causal prompt blocks; same shapes, runtime ``kv_len`` and assertion style as the
 
 from __future__ import annotations
 
+import ctypes
 import functools
 import math
 import struct
@@ -138,6 +139,26 @@ def _workspace_bytes(device_index, *shape) -> int:
     return lib.motif_sdpa_dual_v_tree_workspace_bytes(*shape)
 
 
+_err_words: dict = {}  # device index -> (pinned int32 word, its value through ctypes)
+
+
+def _err_word(dev) -> int | None:
+    """Address of the device's error word, in pinned host memory: a kernel sets it when a pipeline wait runs out, and
+    the next call raises without a synchronisation. A first call under capture, where host memory cannot be
+    pinned, goes without."""
+    known = _err_words.get(dev.index)
+    if known is None:
+        if torch.cuda.is_current_stream_capturing():
+            return None
+        word = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+        known = _err_words[dev.index] = word, ctypes.c_int32.from_address(word.data_ptr())
+    word, value = known
+    if value.value:
+        value.value = 0
+        raise RuntimeError("sdpa_dual_v_tree: a pipeline wait of an earlier call timed out; its rows are NaN")
+    return word.data_ptr()
+
+
 def _launch(q, parts, strides, bits, group_size, scale, HKV, cap, kv_len, tree_mask, name):
     """parts: data, scales, biases of k, v1, v2 in turn (scales and biases None for plain rows)."""
     B, HQ, T, D = q.shape
@@ -158,8 +179,9 @@ def _launch(q, parts, strides, bits, group_size, scale, HKV, cap, kv_len, tree_m
         kv = motif_tree_kv.from_buffer_copy(_KV.pack(*at[0::3], *at[1::3], *at[2::3], *strides))
         ws_bytes = _workspace_bytes(dev.index, code, bits, group_size, B, HQ, HKV, T, cap, D, cap if n_dev else n, 1 - n_step)
         ws = workspace(ws_bytes, dev) if ws_bytes else None
+        err = _err_word(dev)
         check(lib.motif_sdpa_dual_v_tree(code, bits, group_size, qc.data_ptr(), kv, ptr(mask), mask_b, float(scale), B, HQ,
-                                         HKV, T, cap, D, n, n_dev, n_step, y.data_ptr(), ptr(ws), ws_bytes, None,
+                                         HKV, T, cap, D, n, n_dev, n_step, y.data_ptr(), ptr(ws), ws_bytes, err,
                                          stream(dev)), name)
     return y
 
@@ -176,7 +198,8 @@ def sdpa_dual_v_tree(q: torch.Tensor, k: torch.Tensor, v1: torch.Tensor, v2: tor
     appended; ``kv_len`` (default KV_cap) is an int, or an int32 CUDA tensor of one length or one per
     sequence (read on the device). ``tree_mask`` (T, T) or (B, T, T) bool: row t sees tree row j where
     tree_mask[t, j]; None is causal. Every row sees the rows before the tree. Returns (B, H_q, T, 2·D) =
-    cat([SDPA(q,k,v1), SDPA(q,k,v2)], axis=-1), zeros for a row that sees nothing.
+    cat([SDPA(q,k,v1), SDPA(q,k,v2)], axis=-1), zeros for a row that sees nothing. A kernel whose pipeline stalls
+    for half a second gives NaN rows; the next call on the device then raises RuntimeError.
     """
     if _DISABLE:
         return sdpa_dual_v_tree_reference(q, k, v1, v2, scale, kv_len, tree_mask)

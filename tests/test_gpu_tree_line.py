@@ -90,3 +90,65 @@ def test_line_with_broken_drafted_rows(cuda, dtype, bits, gs, bad):
     want, tol = attention64(q, *safe, 0.09, lens, m64, torch.finfo(DT[dtype]).eps / 2, bits != 16)
     assert not torch.isfinite(got[sees]).any()
     check(torch.where(sees, 0.0, got), torch.where(sees, 0.0, want), tol, dtype)
+
+
+def test_a_timed_out_wait_is_raised_by_the_next_call(cuda, monkeypatch):
+    """The failure is made on the host: the library call sets the error word that it was given, as a kernel does
+    whose wait ran out. The next call raises, the one after that is served; captured calls carry the word too."""
+    import ctypes
+
+    from mlx_motif.kernels import tree
+
+    q, kv, _ = make(0, 1, 4, 2, 3, 64, 64, "fp16")
+    want = call(q, kv, 16, 64, 0.1)
+    words = []
+
+    class Lib:
+        def motif_sdpa_dual_v_tree(self, *args):
+            rc = real.motif_sdpa_dual_v_tree(*args)
+            words.append(args[-2])
+            ctypes.c_int32.from_address(args[-2]).value = 1
+            return rc
+
+        def __getattr__(self, name):
+            return getattr(real, name)
+
+    real = tree.lib
+    with monkeypatch.context() as m:
+        m.setattr(tree, "lib", Lib())
+        call(q, kv, 16, 64, 0.1)
+    with pytest.raises(RuntimeError, match="timed out"):
+        call(q, kv, 16, 64, 0.1)
+    assert torch.equal(call(q, kv, 16, 64, 0.1), want)
+    g = torch.cuda.CUDAGraph()
+    with monkeypatch.context() as m, torch.cuda.graph(g):
+        m.setattr(tree, "lib", Lib())
+        call(q, kv, 16, 64, 0.1)
+    assert words[0] == words[1]
+    with pytest.raises(RuntimeError, match="timed out"):
+        call(q, kv, 16, 64, 0.1)
+    g.replay()
+    assert torch.equal(call(q, kv, 16, 64, 0.1), want)
+
+
+def test_first_call_under_capture(cuda):
+    """In a fresh process, the device's first call inside a capture."""
+    import os
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import torch
+from test_gpu_tree import call, make
+q, kv, _ = make(0, 1, 4, 2, 3, 64, 64, "fp16")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y = call(q, kv, 16, 64, 0.1)
+g.replay()
+assert torch.equal(y, call(q, kv, 16, 64, 0.1))
+"""
+    here = Path(__file__).resolve().parent
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join([str(here), str(here.parent / "mlx-motif_b200"), str(here.parent)]))
+    subprocess.run([sys.executable, "-c", code], check=True, env=env, timeout=300)
