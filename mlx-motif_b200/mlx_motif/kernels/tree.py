@@ -55,8 +55,15 @@ def sdpa_dual_v_tree_reference(q, k, v1, v2, scale, kv_len=None, tree_mask=None)
     p = torch.exp(s - torch.where(top == -math.inf, 0.0, top))
     den = p.sum(-1, keepdim=True)
     p = p / torch.where(den == 0, 1.0, den)
-    live = seen.any(1)[:, None, :, None]  # a row nobody sees may hold anything
-    out = [torch.matmul(p, torch.where(live, v, 0.0)) for v in (v1, v2)]
+    out = []
+    for v in (v1, v2):
+        finite = torch.isfinite(v)
+        o = torch.matmul(p, torch.where(finite, v, 0.0))
+        # a row that a query does not see may hold anything: infinities and NaN go to those that see it, row by row
+        for c in (~finite).any(-1).any(0).any(0).nonzero()[:, 0].tolist():
+            rest = torch.where(finite[:, :, c], 0.0, v[:, :, c])[:, :, None]
+            o = o + torch.where(seen[:, None, :, c, None], p[..., c, None] * rest, 0.0)
+        out.append(o)
     return torch.cat(out, dim=-1).to(q.dtype)
 
 
