@@ -63,12 +63,13 @@ def test_line_of_one_tile_units(cuda, D, dtype, bits, gs):
 
 @pytest.mark.parametrize("dtype,bits,gs", TYPES)
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
-def test_line_with_broken_drafted_rows(cuda, dtype, bits, gs, bad):
+@pytest.mark.parametrize("B,cap,kind", [(32, 2000, "mixed"), (160, 112, "short")])  # one to three units a CTA, or nine
+def test_line_with_broken_drafted_rows(cuda, B, cap, kind, dtype, bits, gs, bad):
     """Every third sequence has one drafted row of NaN or infinities, and all rows behind the last are: the
     records of cleared rows are used again by later units of a CTA, and no other row is touched."""
-    B, HQ, HKV, T, D, cap = 32, 24, 8, 5, 128, 2000
+    HQ, HKV, T, D = 24, 8, 5, 128
     rng = np.random.default_rng(7)
-    lens = lengths("mixed", B, T, cap, rng)
+    lens = lengths(kind, B, T, cap, rng)
     q, kv, plain = make(11, B, HQ, HKV, T, D, cap, dtype, bits, gs)
     m, m64 = masks("trees", B, T)
     broken = {b: int(rng.integers(1, T)) for b in range(0, B, 3)}
