@@ -588,8 +588,8 @@ MOTIF_API int motif_speculative_accept(const void* p_logits, const void* q_logit
  * drafted token tokens[b, i] with parent row parents[i] < i ((rows) for all
  * sequences, or (B, rows) with parents_batch_stride = rows). p_logits: the
  * target's row after tree row r; q_logits: the draft's row r, from which row
- * r's children were drawn independently (draft_rows rows: only rows with
- * children are read; a row without a draft row accepts no child). Starting at
+ * r's children were drawn independently (draft_rows rows: what rows without
+ * children hold does not matter; a row without a draft row accepts no child). Starting at
  * row 0 the children of the current row are tested in ascending order with
  * uniforms[b, i]: accepted with probability min(1, w(x) / q(x)), w = p and
  * after each rejection max(0, w - q) renormalised; an accepted child becomes

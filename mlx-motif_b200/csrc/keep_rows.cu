@@ -6,9 +6,9 @@
 // read before it is written, and a later group reads rows ≥ its own j, which no earlier one has written.
 //
 // One launch serves up to kLayers caches: their pointers travel in the kernel's parameters.
-// Bound by the launch: 3 rows of 48 fp16 layers (8 heads, D 128; 2.4 MB read and written) take 2.8 us, 8 rows of 48 q4
-// layers 4.1 us; the bytes alone would be 0.4. A CTA moves one buffer of a slot's head (codes, scales and biases one
-// after the other: 5.2 us); packed rows are short, and CTAs of 64 threads all run at once there (of 128: 5.1 us).
+// Bound by the launch: 3 rows of 48 fp16 layers (8 heads, D 128; 2.4 MB read and written) take 3.2 us, 8 rows of 48 q4
+// layers 4.9 us; the bytes alone would be 0.4. A CTA moves one buffer of a slot's head (codes, scales and biases one
+// after the other: 1.1 us more); packed rows are short, and CTAs of 64 threads all run at once there (of 128: 1.0 us more).
 #include "common.cuh"
 
 namespace motif {

@@ -17,9 +17,9 @@
 //
 // Bound by the rows of k, v1 and v2, each read once (the packed rows share them), until gqa·T is some hundred:
 // 98.7 MB for a tree of 64 over 16064 fp16 rows, 8 kv heads, D 128 (15 us at the copy rate of 6.57 TB/s). Measured
-// there: 41 us, some 27 of it in the tiles (a TMA read of the same rows alone 17.6), 8 start and output, 6 the join;
-// a tree of 17 over 16017 q4 rows 36 us, bound by the instructions that rebuild its tiles (28 MB; floor 4.3); eight
-// ragged requests of 31 rows, 263 MB, 83 us (48 % of the copy rate); a chain of five over 164 rows 8 us, latency.
+// there: 42 us, some 27 of it in the tiles (a TMA read of the same rows alone 17.6), 8 start and output, 6 the join;
+// a tree of 17 over 16017 q4 rows 36 us, bound by the warps that rebuild its tiles (28 MB; floor 4.3); eight
+// ragged requests of 31 rows, 263 MB, 85 us (47 % of the copy rate); a chain of five over 164 rows 8.6 us, latency.
 #include <cooperative_groups.h>
 #include <cuda.h>
 

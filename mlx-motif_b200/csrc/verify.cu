@@ -24,11 +24,11 @@
 //     S_j in 64 bits and exchange the sums through distributed shared memory (each part added in the same
 //     order by everyone, so the CTAs stay in step without another word). The draw finds the CTA, then the
 //     warp's range, then the entry.
-// The walk is bound by latency and by the 64-bit pipes: a pass over a row pair of 219520 entries is 439 k
-// exponentials of nine 64-bit operations on the cluster's SMs.
-// Measured: a tree of 64 over 219520 fp16 entries 30 us (the row sums read 55.8 MB in 13, floor 8.5; the rest is
-// the walk), a chain of five 18 (both rows of every rejection summed once more), 16 trees of nine over 32001 bf16
-// entries 24, a greedy chain of 17 fp32 rows 7.0 (14.9 MB, floor 2.3).
+// The walk is bound by latency, step after step on one cluster: a pass over a row pair of 219520 entries is 439 k
+// exponentials of nine 64-bit operations on the cluster's SMs, whose 64-bit pipes are 12 % active over a walk.
+// Measured: a tree of 64 over 219520 fp16 entries 28 us (the row sums read 55.8 MB in 13, floor 8.5; the rest is
+// the walk), a chain of five 20 (both rows of every rejection summed once more), 16 trees of nine over 32001 bf16
+// entries 25, a greedy chain of 17 fp32 rows 8.3 (14.9 MB, floor 2.3).
 #include <cooperative_groups.h>
 
 #include <atomic>

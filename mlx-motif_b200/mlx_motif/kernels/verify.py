@@ -104,11 +104,12 @@ def speculative_verify(tokens: torch.Tensor, parents: torch.Tensor, p_logits: to
     Row 0 is the last committed token; row i ≥ 1 is drafted token ``tokens[b, i]``, a child of row
     ``parents[…, i]`` < i. tokens (B, T) int32; parents (T,) or (B, T) int32; p_logits (B, T, V), the target's
     row after each tree row; q_logits (B, R, V), R ≤ T, the draft's row r, from which row r's children were
-    drawn independently (rows without children are not read); uniforms (B, T) fp32 in [0, 1): [b, i] tests row
-    i, [b, 0] draws the next token. Children are tested in ascending order: accepted with probability
-    min(1, w(x) / q(x)), w = p, after each rejection w = max(0, w − q) renormalised; the next token is drawn
-    from the last w. At ``temperature`` 0 (q_logits and uniforms may be None) a child is accepted if it is the
-    target's argmax. Returns (accepted, path, next_token) on the device: no synchronisation.
+    drawn independently (what rows without children hold does not matter); uniforms (B, T) fp32 in [0, 1):
+    [b, i] tests row i, [b, 0] draws the next token (from 1 on the last one with weight). Children are tested in
+    ascending order: accepted with probability min(1, w(x) / q(x)), w = p, after each rejection
+    w = max(0, w − q) renormalised; the next token is drawn from the last w. At ``temperature`` 0 (q_logits and
+    uniforms may be None) a child is accepted if it is the target's argmax. Returns (accepted, path, next_token)
+    on the device: no synchronisation.
 
     A token outside [0, V) is never accepted (padding of a smaller tree). NaN logits count as −inf. ``temperature``
     is 0 or in [1e-6, 1e6].
