@@ -126,27 +126,33 @@ int motif_kv4_keep_rows(int dtype, const motif_kv4_slots* caches, int64_t n_cach
   a.base_step = (int32_t)base_stride;
   a.base = base;
   a.T = (int32_t)tree_rows;
-  for (int64_t l0 = 0; l0 < n_caches; l0 += kLayers) {
-    const int n = (int)(n_caches - l0 < kLayers ? n_caches - l0 : kLayers);
-    uintptr_t al[3] = {0, 0, 0};
-    for (int l = 0; l < n; ++l) {
-      const motif_kv4_slots& c = caches[l0 + l];
-      MOTIF_REQUIRE(c.bits == c0.bits && c.group_size == c0.group_size && c.batch == c0.batch && c.heads == c0.heads &&
-                        c.capacity == c0.capacity && c.head_dim == c0.head_dim,
-                    MOTIF_ERR_BAD_SHAPE, "keep_rows: cache %lld differs from the first", (long long)(l0 + l));
-      for (int s = 0; s < 4; ++s) {
-        void* p[3] = {c.data[s], c.scales[s], c.biases[s]};
-        for (int k = 0; k < a.parts; ++k) {
-          MOTIF_REQUIRE(p[k], MOTIF_ERR_NULL, "keep_rows: cache %lld slot %d null", (long long)(l0 + l), s);
-          a.ptr[l][s][k] = p[k];
-          al[k] |= reinterpret_cast<uintptr_t>(p[k]);
-        }
+  uintptr_t al[3] = {0, 0, 0};
+  for (int64_t l = 0; l < n_caches; ++l) {  // all of them before the first launch: a refused call moves nothing
+    const motif_kv4_slots& c = caches[l];
+    MOTIF_REQUIRE(c.bits == c0.bits && c.group_size == c0.group_size && c.batch == c0.batch && c.heads == c0.heads &&
+                      c.capacity == c0.capacity && c.head_dim == c0.head_dim,
+                  MOTIF_ERR_BAD_SHAPE, "keep_rows: cache %lld differs from the first", (long long)l);
+    for (int s = 0; s < 4; ++s) {
+      const void* p[3] = {c.data[s], c.scales[s], c.biases[s]};
+      for (int k = 0; k < a.parts; ++k) {
+        MOTIF_REQUIRE(p[k], MOTIF_ERR_NULL, "keep_rows: cache %lld slot %d null", (long long)l, s);
+        al[k] |= reinterpret_cast<uintptr_t>(p[k]);
       }
     }
-    for (int k = 0; k < a.parts; ++k) {
-      const uintptr_t bits = al[k] | (uintptr_t)a.row_bytes[k];
-      a.unit[k] = bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : 2;
-      MOTIF_REQUIRE(bits % 2 == 0, MOTIF_ERR_BAD_CONTRACT, "keep_rows: misaligned cache");
+  }
+  for (int k = 0; k < a.parts; ++k) {
+    const uintptr_t bits = al[k] | (uintptr_t)a.row_bytes[k];
+    a.unit[k] = bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : 2;
+    MOTIF_REQUIRE(bits % 2 == 0, MOTIF_ERR_BAD_CONTRACT, "keep_rows: misaligned cache");
+  }
+  for (int64_t l0 = 0; l0 < n_caches; l0 += kLayers) {
+    const int n = (int)(n_caches - l0 < kLayers ? n_caches - l0 : kLayers);
+    for (int l = 0; l < n; ++l) {
+      const motif_kv4_slots& c = caches[l0 + l];
+      for (int s = 0; s < 4; ++s) {
+        void* p[3] = {c.data[s], c.scales[s], c.biases[s]};
+        for (int k = 0; k < a.parts; ++k) a.ptr[l][s][k] = p[k];
+      }
     }
     keep_rows_kernel<<<dim3((unsigned)(4 * n), (unsigned)a.heads, (unsigned)a.parts), a.parts == 1 ? kKeepThreads : kKeepThreads / 2, 0, as_stream(stream)>>>(a);
     const int rc = check_launch("keep_rows");
