@@ -91,8 +91,8 @@ int motif_kv4_keep_rows(int dtype, const motif_kv4_slots* caches, int64_t n_cach
                 "keep_rows: unsupported dtype code %d", dtype);
   const motif_kv4_slots& c0 = caches[0];
   MOTIF_REQUIRE(c0.bits == 16 || c0.bits == 4 || c0.bits == 8, MOTIF_ERR_DTYPE, "keep_rows: bits %d", c0.bits);
-  MOTIF_REQUIRE(c0.batch >= 1 && c0.heads >= 1 && c0.capacity >= 1 && c0.head_dim >= 1 &&
-                    c0.batch * c0.heads < 65536,
+  MOTIF_REQUIRE(c0.batch >= 1 && c0.batch < 65536 && c0.heads >= 1 && c0.heads < 65536 && c0.capacity >= 1 &&
+                    c0.head_dim >= 1 && c0.head_dim <= 65536 && c0.batch * c0.heads < 65536,
                 MOTIF_ERR_BAD_SHAPE, "keep_rows: batch=%lld heads=%lld capacity=%lld head_dim=%lld", (long long)c0.batch,
                 (long long)c0.heads, (long long)c0.capacity, (long long)c0.head_dim);
   MOTIF_REQUIRE(row_limit >= 1 && row_limit <= c0.capacity, MOTIF_ERR_BAD_SHAPE,
@@ -105,6 +105,8 @@ int motif_kv4_keep_rows(int dtype, const motif_kv4_slots* caches, int64_t n_cach
   MOTIF_REQUIRE(!base_dev || base_stride == 0 || base_stride == 1, MOTIF_ERR_BAD_SHAPE, "keep_rows: base stride %lld (0 or 1)",
                 (long long)base_stride);
   const int64_t esz = dtype == MOTIF_F32 ? 4 : 2;
+  MOTIF_REQUIRE(tree_rows * c0.head_dim * esz < (1ll << 31), MOTIF_ERR_BAD_SHAPE,  // units of the rows, in 32 bits
+                "keep_rows: %lld rows of %lld channels", (long long)tree_rows, (long long)c0.head_dim);
   KeepArgs a{};
   a.parts = c0.bits == 16 ? 1 : 3;
   if (c0.bits == 16) {
